@@ -318,6 +318,67 @@ SF_API int sf_csc_gather(const int64_t *col_ptr, int64_t n_cols, const int32_t *
                          const sf_matrix *R, const sf_matrix *W, float *dots, const sf_matrix *out,
                          float *col_sums, void *workspace, size_t workspace_bytes, sf_stream stream);
 
+/*
+ * Block-scaled 8-bit matrices. data holds e4m3 numbers [rows, cols] (row pitch data_pitch bytes, a
+ * multiple of 16; base 16-byte aligned); scales holds one power-of-two scale byte s, worth
+ * 2^(s - 127), for each block of SF_BLOCK columns of a row (tile = 0: [rows, nb]) or of SF_BLOCK
+ * rows x SF_BLOCK columns (tile = 1: [ceil(rows / SF_BLOCK), nb]), nb = ceil(cols / SF_BLOCK), row
+ * pitch scale_pitch bytes, a multiple of 4; base 4-byte aligned. Element (i, j) is worth
+ * data[i, j] * 2^(s - 127) of its block. A quantised block has the smallest s whose scale brings its
+ * largest finite magnitude to at most 448, and each element is its quotient by the scale (exact)
+ * rounded once to e4m3, nearest even; an infinity or NaN becomes NaN.
+ */
+#define SF_BLOCK 128
+typedef struct sf_blocks {
+    void *data;
+    void *scales;
+    int64_t rows, cols;
+    int64_t data_pitch, scale_pitch;   /* in bytes */
+    int32_t tile;
+    int32_t reserved;
+} sf_blocks;
+
+/*
+ * Quantises the rows of x [n, cols] (any dtype and strides) into dst (row blocks): row i goes to row
+ * slots[i] of dst, or to row i where slots is NULL. A negative slot drops the row; a slot past
+ * dst->rows is skipped and sets bit 2 of the device error. Slots must be distinct.
+ */
+SF_API int sf_blocks_write(const sf_matrix *x, const int64_t *slots, const sf_blocks *dst, sf_stream stream);
+
+/*
+ * out[i, :] = the dequantised row rows[i] of src (row i where rows is NULL, out->rows rows), in out's
+ * dtype, unit column stride; src in row blocks or tiles. A negative row reads as zeros; one past
+ * src->rows too, and sets bit 2 of the device error.
+ */
+SF_API int sf_blocks_read(const sf_blocks *src, const int64_t *rows, const sf_matrix *out, sf_stream stream);
+
+/* dst[i, :] = src[rows[i], :] as it is held (both in row blocks); rows as in sf_blocks_read. */
+SF_API int sf_blocks_take(const sf_blocks *src, const int64_t *rows, const sf_blocks *dst, sf_stream stream);
+
+/* Bytes of workspace sf_blocks_quantize needs: fp32 partial column sums where they are asked for. */
+SF_API int sf_blocks_quantize_workspace(const sf_matrix *x, int col_sums, size_t *bytes);
+
+/*
+ * Quantises x [R, C] (any dtype and strides) into q (x itself, [R, C]) and qt (its transpose, [C, R]);
+ * either may be NULL. Both are in row blocks, or both in tiles (whose scales are then the same). With
+ * col_sums (fp32 [C], may be NULL) also the sums over the rows of x, in fp32 and in one fixed order.
+ */
+SF_API int sf_blocks_quantize(const sf_matrix *x, const sf_blocks *q, const sf_blocks *qt, float *col_sums,
+                              void *workspace, size_t workspace_bytes, sf_stream stream);
+
+/* Bytes of workspace sf_block_matmul needs for these operands. */
+SF_API int sf_block_matmul_workspace(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out, size_t *bytes);
+
+/*
+ * out = act(a @ b^T + bias): a [M, K] and b [N, K], each in row blocks or tiles; products and scales on
+ * the 8-bit tensor cores, fp32 accumulation. bias (fp32 [N]) may be NULL. activation: enum
+ * sf_activation, or -1 for none; threshold (fp32 [N]) only for SF_ACT_JUMPRELU. out [M, N] in any dtype
+ * and row stride, unit column stride.
+ */
+SF_API int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, const float *threshold,
+                           int activation, const sf_matrix *out, void *workspace, size_t workspace_bytes,
+                           sf_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,8 +5,10 @@ Drop-in for saeflow's `encode / encode_sparse / decode_sparse / forward` and
 """
 
 from .ops import HostForward, decode_sparse, encode, encode_sparse, forward, forward_host, forward_host_async
+from .quantized import QuantizedSAE
 from .sae import SAE
+from .store import ActivationStore
 
 __version__ = "0.1.0"
-__all__ = ["SAE", "HostForward", "decode_sparse", "encode", "encode_sparse", "forward", "forward_host",
-           "forward_host_async"]
+__all__ = ["SAE", "ActivationStore", "HostForward", "QuantizedSAE", "decode_sparse", "encode", "encode_sparse",
+           "forward", "forward_host", "forward_host_async"]

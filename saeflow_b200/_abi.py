@@ -27,6 +27,7 @@ SF_VARIANT_AUTO, SF_VARIANT_TCGEN05, SF_VARIANT_SIMT, SF_VARIANT_TCGEN05_SINGLE 
 SF_OK, SF_ERR_INVALID, SF_ERR_UNSUPPORTED, SF_ERR_CUDA, SF_ERR_WORKSPACE, SF_ERR_DEVICE = range(6)
 ABI_VERSION = 1
 CSR_TILE = 256  # SF_CSR_TILE
+BLOCK = 128  # SF_BLOCK
 
 # Every symbol the header declares, with its ctypes signature.
 _c = ctypes
@@ -44,6 +45,14 @@ class SfVector(_c.Structure):
                 ("len", _c.c_int64), ("stride", _c.c_int64)]
 
 
+class SfBlocks(_c.Structure):
+    _fields_ = [("data", _c.c_void_p), ("scales", _c.c_void_p),
+                ("rows", _c.c_int64), ("cols", _c.c_int64),
+                ("data_pitch", _c.c_int64), ("scale_pitch", _c.c_int64),
+                ("tile", _c.c_int32), ("reserved", _c.c_int32)]
+
+
+_BP = _c.POINTER(SfBlocks)
 _MP = _c.POINTER(SfMatrix)
 _VP = _c.POINTER(SfVector)
 _SIZE_P = _c.POINTER(_c.c_size_t)
@@ -74,6 +83,13 @@ SIGNATURES = {
     "sf_csc_gather_workspace": (_c.c_int, [_c.c_int64, _MP, _SIZE_P]),
     "sf_csc_gather": (_c.c_int, [_P, _c.c_int64, _P, _c.c_int64, _P, _P, _P, _c.c_int, _MP, _MP, _P, _MP, _P, _P,
                                  _c.c_size_t, _P]),
+    "sf_blocks_write": (_c.c_int, [_MP, _P, _BP, _P]),
+    "sf_blocks_read": (_c.c_int, [_BP, _P, _MP, _P]),
+    "sf_blocks_take": (_c.c_int, [_BP, _P, _BP, _P]),
+    "sf_blocks_quantize_workspace": (_c.c_int, [_MP, _c.c_int, _SIZE_P]),
+    "sf_blocks_quantize": (_c.c_int, [_MP, _BP, _BP, _P, _P, _c.c_size_t, _P]),
+    "sf_block_matmul_workspace": (_c.c_int, [_BP, _BP, _MP, _SIZE_P]),
+    "sf_block_matmul": (_c.c_int, [_BP, _BP, _P, _P, _c.c_int, _MP, _P, _c.c_size_t, _P]),
     "sf_topk_encode_workspace": (_c.c_int, [_MP, _MP, _c.c_int, _c.c_int, _SIZE_P]),
     "sf_topk_encode": (_c.c_int, [_MP, _MP, _VP, _VP, _c.c_int, _P, _P, _c.c_int, _c.c_int, _P,
                                   _c.c_size_t, _P]),

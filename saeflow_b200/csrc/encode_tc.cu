@@ -1248,13 +1248,10 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_tiled() {
     return fn;
 }
 
-int make_map_2d(CUtensorMap *map, const void *base, int ab_fmt, uint64_t inner, uint64_t outer,
+int make_map_of(CUtensorMap *map, const void *base, CUtensorMapDataType dt, uint64_t inner, uint64_t outer,
                 uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer) {
     auto fn = get_encode_tiled();
     if (!fn) return set_error(SF_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-    const CUtensorMapDataType dt = ab_fmt == 2   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : ab_fmt == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     cuuint64_t dims[2] = {inner, outer};
     cuuint64_t strides[1] = {row_pitch_bytes};
     cuuint32_t box[2] = {box_inner, box_outer};
@@ -1266,6 +1263,14 @@ int make_map_2d(CUtensorMap *map, const void *base, int ab_fmt, uint64_t inner, 
         return set_error(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) inner=%llu outer=%llu pitch=%llu", (int)r,
                          (unsigned long long)inner, (unsigned long long)outer, (unsigned long long)row_pitch_bytes);
     return SF_OK;
+}
+
+int make_map_2d(CUtensorMap *map, const void *base, int ab_fmt, uint64_t inner, uint64_t outer,
+                uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer) {
+    const CUtensorMapDataType dt = ab_fmt == 2   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : ab_fmt == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return make_map_of(map, base, dt, inner, outer, row_pitch_bytes, box_inner, box_outer);
 }
 
 template <int AB_FMT, bool B_MN, int MODE, int STAGES, bool PART>
@@ -1366,6 +1371,11 @@ void fill_common(TcParams &p, const GemmOperands &g, bool pair, unsigned *err) {
 }
 
 }  // namespace
+
+int make_map_e4m3(CUtensorMap *map, const void *base, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
+                  uint32_t box_rows) {
+    return make_map_of(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, cols, rows, pitch_bytes, 128, box_rows);
+}
 
 // Pairs of SMs that can hold one pair-kernel cluster each (cached per kernel).
 int pair_slots(const void *kern, const cudaLaunchConfig_t &cfg) {

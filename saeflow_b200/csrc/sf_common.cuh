@@ -297,6 +297,23 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// D (+)= (A * scale_a) (B * scale_b)^T on e4m3 operands with one e8m0 scale byte per row and 32
+// elements of K, held in TMEM (kind::mxf8f6f4): 32 elements of K per instruction.
+__device__ __forceinline__ void umma_e4m3_scaled(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                 uint32_t scale_a_tmem, uint32_t scale_b_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(scale_a_tmem), "r"(scale_b_tmem), "r"(accumulate)
+        : "memory");
+}
+// 32 rows x 16 bytes of shared memory into four TMEM columns of lanes 0..31, repeated for each of
+// the four warps' lanes: the layout the scale operands are read in.
+__device__ __forceinline__ void tmem_copy_32x128b(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 // ---------------------------------------------------------------------------------------
 // Thread-block clusters and the CTA pair of cta_group::2
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -403,6 +420,24 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t ab_format, bool b_mn_major, int M, int N) {
     return (1u << 4) | (ab_format << 7) | (ab_format << 10) | (0u << 15) | ((b_mn_major ? 1u : 0u) << 16) |
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// Shared-memory descriptor without a swizzle (layout code 0): 8-row groups of 16-byte rows, 128
+// bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((128u >> 4) & 0x3FFFu) << 32;
+    d |= 1ull << 46;
+    return d;
+}
+
+// Instruction descriptor for kind::mxf8f6f4 with e4m3 operands (formats 0), K-major both, e8m0 scales:
+//   B scale byte [4,6); N>>3 at [17,23); scale format bit 23 = 1 (E8M0); M>>4 at [24,29); A scale byte
+//   [29,31). The scale bytes pick one of the four bytes of the scale operands' 32-bit words.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3_scaled(int M, int N, uint32_t scale_byte) {
+    return (scale_byte << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+           (static_cast<uint32_t>(M >> 4) << 24) | (scale_byte << 29);
 }
 
 // ---------------------------------------------------------------------------------------

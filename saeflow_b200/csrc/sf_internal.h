@@ -1,10 +1,13 @@
 // Host-side interfaces between the saeflow_b200 translation units.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
+
+#include "saeflow_b200.h"
 
 namespace sf {
 
@@ -131,6 +134,11 @@ constexpr int kCsrTile = 256;  // columns per (row, tile) count cell
 
 int encode_tc_dense(const GemmOperands &g, const EpilogueArgs &ep, int variant, cudaStream_t stream);
 int encode_tc_csr(const GemmOperands &g, const EpilogueArgs &ep, const CsrArgs &csr, cudaStream_t stream);
+// Tensor map of a row-major matrix of 8-bit numbers: boxes of box_rows rows x 128 bytes, 128-byte
+// swizzle, zeros past the extents (encode_tc.cu).
+int make_map_e4m3(CUtensorMap *map, const void *base, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
+                  uint32_t box_rows);
+int check_blocks(const sf_blocks *b, const char *name);
 int pair_slots(const void *kern, const cudaLaunchConfig_t &cfg);
 int encode_tc_topk(const GemmOperands &g, const TopkArgs &tk, cudaStream_t stream);
 int topk_chunks(int64_t M, int64_t N);

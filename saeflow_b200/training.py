@@ -30,6 +30,7 @@ import torch
 
 from .kernels import sparse_decode
 from .kernels.backward import csc_gather, csr_sddmm, csr_transpose, matvec, transpose
+from .kernels.blocks import BlockScaled, block_matmul, quantize_both
 
 
 @dataclass
@@ -99,3 +100,54 @@ def forward(sae, x):
     threshold, activation, k), e.g. saeflow_b200.SAE with requires_grad parameters."""
     return _SparseForward.apply(x, sae.W_enc, sae.b_enc, sae.W_dec, sae.b_dec, getattr(sae, "threshold", None),
                                 sae.activation, getattr(sae, "k", None))
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, W, b):
+        need_x, need_W = ctx.needs_input_grad[:2]
+        xq, xt, _ = quantize_both(x.detach(), want=(True, need_W))
+        wq, wt, _ = quantize_both(W.detach(), tile=True, want=(need_x, True))
+        # two tensors each for what the backward reads: autograd keeps and frees them
+        ctx.save_for_backward(*(t for m in (xt, wq) if m is not None for t in (m.data, m.scales)))
+        ctx.dtypes = x.dtype, W.dtype, None if b is None else b.dtype
+        ctx.shapes = x.shape, W.shape
+        return block_matmul(xq, wt, b, out_dtype=x.dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        need_x, need_W, need_b = ctx.needs_input_grad[:3]
+        saved = list(ctx.saved_tensors)
+        xt = BlockScaled(saved.pop(0), saved.pop(0)) if need_W else None
+        wq = BlockScaled(saved.pop(0), saved.pop(0), tile=True) if need_x else None
+        x_dtype, W_dtype, b_dtype = ctx.dtypes
+        dx = dW = db = None
+        if not dy.shape[0]:
+            (x_shape, W_shape) = ctx.shapes
+            dx = dy.new_zeros(x_shape, dtype=x_dtype) if need_x else None
+            dW = dy.new_zeros(W_shape, dtype=W_dtype) if need_W else None
+            return dx, dW, dy.new_zeros(dy.shape[1], dtype=b_dtype) if need_b else None
+        if need_x or need_W or need_b:
+            dyq, dyt, sums = quantize_both(dy, want=(need_x or not need_W, need_W), col_sums=need_b)
+            dx = block_matmul(dyq, wq, out_dtype=x_dtype) if need_x else None
+            dW = block_matmul(xt, dyt, out_dtype=W_dtype) if need_W else None
+            db = sums.to(b_dtype) if need_b else None
+        return dx, dW, db
+
+
+def linear8(x, W, b=None):
+    """x @ W + b on the 8-bit tensor cores, differentiable in x, W and b: for SAEs (or phases of their
+    training) whose features are dense, where `forward`'s sparse backward has nothing to skip.
+
+    x [M, K], W [K, N] (the orientation of W_enc and W_dec), b [N] or None; fp32 / bf16 / fp16. Every
+    product is of operands quantised to e4m3 with a power-of-two scale per block of 128 along the axis
+    it sums over (W: per 128 x 128 tile), accumulated in fp32, rounded once to the dtype of what it
+    computes (y and dx: x's, dW: W's):
+        y  = Q(x) @ Q(W) + b        dx = Q(dy) @ Q(W)^T
+        dW = Q(x^T) @ Q(dy^T)^T     db = sum_rows dy   (dy as it is, fp32, in a fixed order)
+    The quantisation itself is taken as the identity (straight through)."""
+    if x.dim() != 2 or W.dim() != 2 or x.shape[1] != W.shape[0]:
+        raise ValueError(f"linear8 takes x [M, K] and W [K, N], got {tuple(x.shape)} and {tuple(W.shape)}")
+    if b is not None and tuple(b.shape) != (W.shape[1],):
+        raise ValueError(f"b must be [{W.shape[1]}], got {tuple(b.shape)}")
+    return _Linear8.apply(x, W, b)
