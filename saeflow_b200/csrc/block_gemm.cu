@@ -8,12 +8,19 @@
 // the instruction descriptor says which byte of the word applies. Tiles (one scale per 128 x 128) are
 // the same words read once per 128 rows.
 //
-// Persistent kernel, one CTA per SM, 128 x 128 tiles, 224 threads:
-//   warp 0      TMA producer: 128 rows x 128 bytes of a and of b per stage, SWIZZLE_128B, mbarrier ring
-//   warp 1      TMEM allocator and MMA issuer; two accumulators of 128 columns
+// Persistent kernel, one CTA per SM, warp-specialised (224 threads):
+//   warp 0      TMA producer: 128-byte rows of both operands, SWIZZLE_128B, mbarrier ring
+//   warp 1      TMEM allocator and MMA issuer
 //   warps 2-5   epilogue: bias, activation, rounding, stores
 //   warp 6      scale words of both operands for 512 elements of K into shared memory, in the order that
 //               tcgen05.cp spreads over TMEM (row r at byte 16 (r % 32) + 4 (r / 32))
+//
+// Two sizes. PAIR: a CTA pair (cta_group::2) computes 256 x 256, each CTA loading 128 rows of either
+// operand; both CTAs' loads complete on the leader's barriers. Single: one CTA computes 128 x COLS.
+// Two orientations. The rows of a tile (TMEM lanes) are rows of `a` and its columns rows of `b`; or,
+// SWAP, the other way round: then a warp's store is 32 neighbouring elements of one output row, which
+// suits outputs whose rows TMA cannot address, and few rows of `a` make a narrow tile (COLS = 32) beside
+// 128 rows of weights.
 #include <algorithm>
 
 #include "sf_common.cuh"
@@ -23,49 +30,79 @@ namespace sf {
 
 namespace {
 
-constexpr int kTile = 128;
-constexpr int kKBytes = 128;                  // elements (bytes) of K per stage
-constexpr int kStages = 6;
-constexpr int kScaleSlots = 4;                // scale words of 512 elements of K each
+constexpr int kKBytes = 128;                   // elements (bytes) of K per stage
+constexpr int kScaleSlots = 3;                 // scale words of 512 elements of K each
 constexpr int kThreads = 224;
-constexpr int kTileBytes = kTile * kKBytes;   // one operand of one stage
 constexpr int kTmemCols = 512;
-constexpr int kScaleCol = 256;                // TMEM columns of the scales, behind the accumulators
+constexpr int kRowTile = 128;                  // rows (TMEM lanes) per CTA
+constexpr int kStageOutBytes = 4096;           // 32 output rows x 128 bytes of one epilogue warp
 
 struct GemmParams {
-    int M, N, nkb;
-    int m_tiles, n_tiles;
-    int group_m;  // m-tiles that run side by side over each n-tile
-    const uint8_t *a_scales, *b_scales;
-    int64_t a_scale_pitch, b_scale_pitch;
-    int a_shift, b_shift;  // log2 of the rows a scale row serves: 0 row blocks, 7 tiles
+    int rows, cols;            // of the tile grid: a's and b's, or b's and a's with SWAP
+    int nkb, groups;           // K blocks of 128, and groups of four of them
+    int splits, split_groups;  // ranges of K: split z takes groups [z split_groups, (z + 1) split_groups)
+    int row_tiles, col_tiles;
+    int group_rows;            // row tiles that run side by side over each column tile
+    const uint8_t *r_scales, *c_scales;  // of the rows' and the columns' operand
+    int64_t r_pitch, c_pitch;
+    int r_shift, c_shift;      // log2 of the rows a scale row serves: 0 row blocks, 7 tiles
     const float *bias, *thr;
-    int activation;  // enum sf_activation, -1 none
-    void *out;
+    int activation;            // enum sf_activation, -1 none
+    void *out;                 // SWAP: plain stores
     int64_t out_pitch;
-    int out_vec;
+    int64_t out_split;         // elements between the splits' outputs
     unsigned *err;
 };
 
+// Compile-time shape of a kernel.
+template <bool PAIR_, int COLS_, int STAGES_>
+struct Shape {
+    static constexpr bool PAIR = PAIR_;
+    static constexpr int COLS = COLS_;                          // columns of a tile
+    static constexpr int ROWS = PAIR ? 256 : 128;               // rows of a tile
+    static constexpr int COLS_HERE = PAIR ? COLS / 2 : COLS;    // rows of the columns' operand loaded per CTA
+    static constexpr int STAGES = STAGES_;
+    static constexpr int R_BYTES = kRowTile * kKBytes, C_BYTES = COLS_HERE * kKBytes;
+    static constexpr int COL_WORDS = COLS <= 128 ? 4 : COLS / 32;  // TMEM columns of the columns' scales
+    static constexpr int SLOT_COLS = 4 + COL_WORDS;
+    static constexpr int SLOT_BYTES = 512 + COL_WORDS / 4 * 512;
+    // Two accumulators and the scales in 512 columns: at 256 columns the accumulators overlap by 40.
+    static constexpr int ACC1 = COLS == 256 ? 216 : COLS;
+    static constexpr int SCALE_COL = ACC1 + COLS;
+    static_assert(SCALE_COL + kScaleSlots * SLOT_COLS <= kTmemCols, "TMEM columns");
+};
+
 struct __align__(16) Shared {
-    uint64_t full[kStages], empty[kStages];
+    uint64_t full[12], empty[12];
     uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];
     uint64_t tmem_full[2], tmem_empty[2];
     uint64_t drain;
     uint32_t tmem_base;
     int abort_flag;
-    alignas(16) float bias[2][kTile];
-    alignas(16) float thr[2][kTile];
+    alignas(16) float bias[2][256];
+    alignas(16) float thr[2][256];
 };
 
-__device__ __forceinline__ void tile_coords(const GemmParams &p, int u, int &m_blk, int &n_blk) {
-    const int per_group = p.group_m * p.n_tiles;
+struct Unit {
+    int row0, col0, split, kb0, kb1;
+};
+
+template <typename S>
+__device__ __forceinline__ Unit unit_of(const GemmParams &p, int u) {
+    Unit r;
+    const int tiles = p.row_tiles * p.col_tiles;
+    r.split = u / tiles;
+    u -= r.split * tiles;
+    const int per_group = p.group_rows * p.col_tiles;
     const int g = u / per_group;
-    const int first = g * p.group_m;
-    const int gm = min(p.m_tiles - first, p.group_m);
+    const int first = g * p.group_rows;
+    const int gm = min(p.row_tiles - first, p.group_rows);
     const int local = u - g * per_group;
-    m_blk = first + local % gm;
-    n_blk = local / gm;
+    r.row0 = (first + local % gm) * S::ROWS;
+    r.col0 = local / gm * S::COLS;
+    r.kb0 = 4 * r.split * p.split_groups;
+    r.kb1 = min(p.nkb, r.kb0 + 4 * p.split_groups);
+    return r;
 }
 
 // The scale words of 128 rows from `first` for K blocks 4 g .. 4 g + 3: lane i gets rows i, 32 + i, 64 + i,
@@ -87,200 +124,330 @@ __device__ __forceinline__ float activate(float v, float t, int activation) {
     return v;
 }
 
-template <typename OT>
-__device__ __forceinline__ void store_chunk(const GemmParams &p, const float (&v)[32], int row, int col0,
-                                            uint64_t policy) {
-    if (row >= p.M) return;
-    OT *dst = reinterpret_cast<OT *>(p.out) + (int64_t)row * p.out_pitch + col0;
-    if (p.out_vec && col0 + 32 <= p.N) {
-        alignas(16) OT o[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = from_f32<OT>(v[j]);
-        const uint4 *src = reinterpret_cast<const uint4 *>(o);
-#pragma unroll
-        for (int j = 0; j < (int)(2 * sizeof(OT)); ++j)
-            st_global_v4_hint(reinterpret_cast<uint4 *>(dst) + j, src[j], policy);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (col0 + j < p.N) dst[j] = from_f32<OT>(v[j]);
-    }
-}
-
-template <typename OT>
+template <typename OT, typename S, bool SWAP>
 __global__ void __launch_bounds__(kThreads, 1)
-    block_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                      const GemmParams p) {
+    block_gemm_kernel(const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmC,
+                      const __grid_constant__ CUtensorMap tmOut, const GemmParams p) {
+    constexpr bool PAIR = S::PAIR;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *sA = smem;
-    uint8_t *sB = sA + kStages * kTileBytes;
-    uint8_t *sScale = sB + kStages * kTileBytes;  // per slot: 512 bytes of a's words, 512 of b's
-    Shared *sh = reinterpret_cast<Shared *>(sScale + kScaleSlots * 1024);
+    uint8_t *sR = smem;
+    uint8_t *sC = sR + S::STAGES * S::R_BYTES;
+    uint8_t *sOut = sC + S::STAGES * S::C_BYTES;  // 4 warps x 2 buffers (not with SWAP)
+    uint8_t *sScale = sOut + (SWAP ? 0 : 8 * kStageOutBytes);
+    Shared *sh = reinterpret_cast<Shared *>(sScale + kScaleSlots * S::SLOT_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int units = p.m_tiles * p.n_tiles;
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+    const bool leader = rank == 0;
+    const int first_unit = PAIR ? (int)cluster_id_x() : (int)blockIdx.x;
+    const int step_units = PAIR ? (int)num_clusters_x() : (int)gridDim.x;
+    const int units = p.row_tiles * p.col_tiles * p.splits;
+    constexpr int kCtas = PAIR ? 2 : 1;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(&sh->full[s], 1);
-            mbar_init(&sh->empty[s], 1);
+        for (int s = 0; s < S::STAGES; ++s) {
+            mbar_init(&sh->full[s], 1);   // leader's: its expect_tx arrive + both CTAs' bytes
+            mbar_init(&sh->empty[s], 1);  // one commit of the leader's MMA thread
         }
         for (int s = 0; s < kScaleSlots; ++s) {
-            mbar_init(&sh->scale_full[s], 1);
+            mbar_init(&sh->scale_full[s], kCtas);  // leader's: one arrive per CTA's scale warp
             mbar_init(&sh->scale_empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sh->tmem_full[b], 1);
-            mbar_init(&sh->tmem_empty[b], 4);
+            mbar_init(&sh->tmem_empty[b], 4 * kCtas);  // leader's: one arrive per epilogue warp
         }
         mbar_init(&sh->drain, 1);
         sh->abort_flag = 0;
         fence_mbar_init();
-        tma_prefetch_desc(&tmA);
-        tma_prefetch_desc(&tmB);
+        tma_prefetch_desc(&tmR);
+        tma_prefetch_desc(&tmC);
+        if (!SWAP) tma_prefetch_desc(&tmOut);
     }
     if (warp == 1) {
-        tmem_alloc(&sh->tmem_base, kTmemCols);
-        tmem_relinquish();
+        if (PAIR) {
+            tmem_alloc_pair(&sh->tmem_base, kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(&sh->tmem_base, kTmemCols);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
-    __syncthreads();
+    if (PAIR)
+        cluster_sync();
+    else
+        __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh->tmem_base;
     volatile int *abort_flag = &sh->abort_flag;
-    auto wait = [&](uint64_t *bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.err); };
+    const uint32_t peer_abort = PAIR ? map_to_rank(smem_u32(&sh->abort_flag), rank ^ 1u) : 0u;
+    // A wait that runs out (or sees the abort flag) also raises the other CTA's flag.
+    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+        if (mbar_wait(bar, parity, abort_flag, p.err)) return true;
+        if (PAIR) st_remote_u32(peer_abort, 1u);
+        return false;
+    };
+    // The same with cluster-scope acquire, for phases that the peer's threads complete.
+    auto wait_cluster = [&](uint64_t *bar, uint32_t parity) -> bool {
+        if (!PAIR) return wait(bar, parity);
+        if (mbar_wait_cluster(bar, parity, abort_flag, p.err)) return true;
+        st_remote_u32(peer_abort, 1u);
+        return false;
+    };
+    auto arrive_leader = [&](uint64_t *bar) {
+        if (PAIR)
+            mbar_arrive_remote(map_to_rank(smem_u32(bar), 0));
+        else
+            mbar_arrive(bar);
+    };
+    // Completion of the MMA thread's work so far, on this barrier of every CTA.
+    auto commit = [&](uint64_t *bar) {
+        if (PAIR) {
+            umma_commit_pair(map_to_rank(smem_u32(bar), 0));
+            umma_commit_pair(map_to_rank(smem_u32(bar), 1));
+        } else {
+            umma_commit(bar);
+        }
+    };
 
     if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer
         if (lane == 0) {
-            const uint64_t pol_a = l2_policy_evict_last(), pol_b = l2_policy_evict_normal();
+            // a group's row tiles are read again for each of its column tiles
+            const uint64_t pol_c = l2_policy_evict_normal();
+            const uint64_t pol_r = p.col_tiles > 1 ? l2_policy_evict_last() : pol_c;
             int stage = 0;
             uint32_t phase = 0, armed = 0, armed_parity = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                int m_blk, n_blk;
-                tile_coords(p, u, m_blk, n_blk);
-                for (int kb = 0; kb < p.nkb; ++kb) {
+            for (int u = first_unit; ok && u < units; u += step_units) {
+                const Unit un = unit_of<S>(p, u);
+                const int row0 = un.row0 + (int)rank * kRowTile, col0 = un.col0 + (int)rank * S::COLS_HERE;
+                for (int kb = un.kb0; kb < un.kb1; ++kb) {
                     if (!(ok = wait(&sh->empty[stage], phase ^ 1u))) break;
-                    mbar_arrive_expect_tx(&sh->full[stage], 2 * kTileBytes);
-                    armed |= 1u << stage;
-                    armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-                    tma_load_2d(sA + stage * kTileBytes, &tmA, &sh->full[stage], kb * kKBytes, m_blk * kTile, pol_a);
-                    tma_load_2d(sB + stage * kTileBytes, &tmB, &sh->full[stage], kb * kKBytes, n_blk * kTile, pol_b);
-                    if (++stage == kStages) {
+                    if (leader) {
+                        mbar_arrive_expect_tx(&sh->full[stage], kCtas * (S::R_BYTES + S::C_BYTES));
+                        armed |= 1u << stage;
+                        armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
+                    }
+                    uint8_t *dr = sR + stage * S::R_BYTES, *dc = sC + stage * S::C_BYTES;
+                    if (PAIR) {
+                        const uint32_t full = map_to_rank(smem_u32(&sh->full[stage]), 0);
+                        tma_load_2d_pair(dr, &tmR, full, kb * kKBytes, row0, pol_r);
+                        tma_load_2d_pair(dc, &tmC, full, kb * kKBytes, col0, pol_c);
+                    } else {
+                        tma_load_2d(dr, &tmR, &sh->full[stage], kb * kKBytes, row0, pol_r);
+                        tma_load_2d(dc, &tmC, &sh->full[stage], kb * kKBytes, col0, pol_c);
+                    }
+                    if (++stage == S::STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
-            if (*abort_flag)  // copies in flight must land before the CTA leaves
-                for (int s = 0; s < kStages; ++s)
-                    if (armed & (1u << s)) mbar_wait_drain(&sh->full[s], (armed_parity >> s) & 1u, p.err);
+            if (*abort_flag) {  // copies in flight must land before the CTA leaves
+                if (leader) {
+                    for (int s = 0; s < S::STAGES; ++s)
+                        if (armed & (1u << s)) mbar_wait_drain(&sh->full[s], (armed_parity >> s) & 1u, p.err);
+                } else {
+                    const unsigned long long t0 = global_timer_ns();
+                    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+                }
+            }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        // ---------------------------------------------------------------- MMA issuer (the leader's)
+        if (leader && lane == 0) {
             int stage = 0, slot = 0, acc = 0;
             uint32_t phase = 0, slot_phase = 0, acc_phase = 0;
-            bool ok = true;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                if (!(ok = wait(&sh->tmem_empty[acc], acc_phase ^ 1u))) break;
+            bool ok = true, first_tile = true;
+            for (int u = first_unit; ok && u < units; u += step_units) {
+                const Unit un = unit_of<S>(p, u);
+                // Accumulators that overlap: the previous tile's epilogue must have read the columns that
+                // this tile's shares with it (and so has finished the tile before that).
+                if (S::ACC1 < S::COLS) {
+                    if (!first_tile && !(ok = wait(&sh->tmem_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1u))) break;
+                    first_tile = false;
+                } else if (!(ok = wait(&sh->tmem_empty[acc], acc_phase ^ 1u))) {
+                    break;
+                }
                 tc_fence_after();
-                const uint32_t d = tmem + acc * kTile;
+                const uint32_t d = tmem + acc * S::ACC1;
                 uint32_t scales = 0;
-                for (int kb = 0; kb < p.nkb; ++kb) {
+                for (int kb = un.kb0; kb < un.kb1; ++kb) {
                     if ((kb & 3) == 0) {
-                        if (!(ok = wait(&sh->scale_full[slot], slot_phase))) break;
+                        if (!(ok = wait_cluster(&sh->scale_full[slot], slot_phase))) break;
                         tc_fence_after();
-                        // Slot by slot: a slot's TMEM columns are written again four slots (16 stages)
-                        // later, when the stages that read them have long been released.
-                        scales = tmem + kScaleCol + slot * 8;
-                        const uint32_t src = smem_u32(sScale + slot * 1024);
-                        tmem_copy_32x128b(scales, smem_desc_rows16(src));
-                        tmem_copy_32x128b(scales + 4, smem_desc_rows16(src + 512));
-                        umma_commit(&sh->scale_empty[slot]);
+                        scales = tmem + S::SCALE_COL + slot * S::SLOT_COLS;
+                        const uint32_t src = smem_u32(sScale + slot * S::SLOT_BYTES);
+#pragma unroll
+                        for (int i = 0; i < S::SLOT_COLS / 4; ++i) {
+                            if (PAIR)
+                                tmem_copy_32x128b_pair(scales + 4 * i, smem_desc_rows16(src + 512 * i));
+                            else
+                                tmem_copy_32x128b(scales + 4 * i, smem_desc_rows16(src + 512 * i));
+                        }
+                    }
+                    if (!(ok = wait(&sh->full[stage], phase))) break;
+                    tc_fence_after();
+                    const uint32_t r = smem_u32(sR + stage * S::R_BYTES), c = smem_u32(sC + stage * S::C_BYTES);
+                    const uint32_t idesc = make_idesc_e4m3_scaled(S::ROWS, S::COLS, kb & 3);
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint64_t rd = smem_desc_sw128(r + ks * 32, 16, 1024);
+                        const uint64_t cd = smem_desc_sw128(c + ks * 32, 16, 1024);
+                        const uint32_t accumulate = (kb > un.kb0 || ks) ? 1u : 0u;
+                        if (PAIR)
+                            umma_e4m3_scaled_pair(d, rd, cd, idesc, scales, scales + 4, accumulate);
+                        else
+                            umma_e4m3_scaled(d, rd, cd, idesc, scales, scales + 4, accumulate);
+                    }
+                    commit(&sh->empty[stage]);
+                    if (++stage == S::STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    // Released with the group's last MMA: a slot is filled again, in shared memory and
+                    // then in TMEM, only after the MMAs that read it.
+                    if ((kb & 3) == 3 || kb + 1 == un.kb1) {
+                        commit(&sh->scale_empty[slot]);
                         if (++slot == kScaleSlots) {
                             slot = 0;
                             slot_phase ^= 1u;
                         }
                     }
-                    if (!(ok = wait(&sh->full[stage], phase))) break;
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(sA + stage * kTileBytes), b = smem_u32(sB + stage * kTileBytes);
-                    const uint32_t idesc = make_idesc_e4m3_scaled(kTile, kTile, kb & 3);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        umma_e4m3_scaled(d, smem_desc_sw128(a + ks * 32, 16, 1024),
-                                         smem_desc_sw128(b + ks * 32, 16, 1024), idesc, scales, scales + 4,
-                                         (kb | ks) ? 1u : 0u);
-                    umma_commit(&sh->empty[stage]);
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
                 }
                 if (!ok) break;
-                umma_commit(&sh->tmem_full[acc]);
+                commit(&sh->tmem_full[acc]);
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
             }
-            umma_commit(&sh->drain);
+            if (PAIR)
+                umma_commit_pair(map_to_rank(smem_u32(&sh->drain), 0));
+            else
+                umma_commit(&sh->drain);
             mbar_wait_drain(&sh->drain, 0, p.err);
         }
     } else if (warp < 6) {
+        // ---------------------------------------------------------------- epilogue
         const int et = threadIdx.x - 64;
         const int quad = warp & 3;
-        const uint64_t pol = l2_policy_evict_first();
+        constexpr int STEP = 64;  // columns loaded at a time
+        constexpr int STEPS = (S::COLS + STEP - 1) / STEP;
+        constexpr int HALVES = S::COLS < STEP ? 1 : 2;
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
-            int m_blk, n_blk;
-            tile_coords(p, u, m_blk, n_blk);
-            const int col = n_blk * kTile + et;
-            sh->bias[acc][et] = p.bias && col < p.N ? __ldg(p.bias + col) : 0.f;
-            sh->thr[acc][et] = p.thr && col < p.N ? __ldg(p.thr + col) : 0.f;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+        int stores = 0;
+        for (int u = first_unit; u < units; u += step_units) {
+            const Unit un = unit_of<S>(p, u);
+            const int row = un.row0 + (int)rank * kRowTile + quad * 32 + lane;
+            float row_bias = 0.f, row_thr = 0.f;
+            if (SWAP) {
+                if (p.bias && row < p.rows) row_bias = __ldg(p.bias + row);
+                if (p.thr && row < p.rows) row_thr = __ldg(p.thr + row);
+            } else {
+                for (int j = et; j < S::COLS; j += 128) {
+                    const int col = un.col0 + j;
+                    sh->bias[acc][j] = p.bias && col < p.cols ? __ldg(p.bias + col) : 0.f;
+                    sh->thr[acc][j] = p.thr && col < p.cols ? __ldg(p.thr + col) : 0.f;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
             if (!wait(&sh->tmem_full[acc], acc_phase)) break;
             tc_fence_after();
-            const int row = m_blk * kTile + quad * 32 + lane;
+            const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1;
+            // Overlapping accumulators: the shared columns (the first's last 40, the second's first 40) are
+            // read first and released to the next tile's MMAs.
+            const int first = S::ACC1 < S::COLS && acc == 0 ? STEPS - 1 : 0;
 #pragma unroll 1
-            for (int c = 0; c < kTile; c += 32) {
-                uint32_t r[32];
-                tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * kTile + c, r);
+            for (int i = 0; i < STEPS; ++i) {
+                const int c0 = (first + i) % STEPS * STEP;
+                uint32_t r[HALVES][32];
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
                 tmem_ld_wait();
-                if (c + 32 == kTile) {
+                if (i == (S::ACC1 < S::COLS ? 0 : STEPS - 1)) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh->tmem_empty[acc]);
+                    if (lane == 0) arrive_leader(&sh->tmem_empty[acc]);
                 }
-                float v[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    v[j] = activate(__uint_as_float(r[j]) + sh->bias[acc][c + j], sh->thr[acc][c + j], p.activation);
-                store_chunk<OT>(p, v, row, n_blk * kTile + c, pol);
+                for (int h = 0; h < HALVES; ++h) {
+                    const int c = c0 + 32 * h;
+                    if constexpr (SWAP) {
+                        if (row < p.rows) {
+                            OT *dst = reinterpret_cast<OT *>(p.out) + un.split * p.out_split +
+                                      (int64_t)(un.col0 + c) * p.out_pitch + row;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                if (un.col0 + c + j < p.cols)
+                                    dst[j * p.out_pitch] = from_f32<OT>(
+                                        activate(__uint_as_float(r[h][j]) + row_bias, row_thr, p.activation));
+                            }
+                        }
+                    } else {
+                        alignas(16) OT o[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            o[j] = from_f32<OT>(activate(__uint_as_float(r[h][j]) + sh->bias[acc][c + j],
+                                                         sh->thr[acc][c + j], p.activation));
+                        // 32 rows x 128 bytes, 16-byte chunk j of row r at chunk j ^ (r % 8): 32 columns of fp32,
+                        // or both halves of 16-bit outputs
+                        constexpr int CHUNKS = 2 * sizeof(OT);
+                        uint8_t *buf = sOut + ((warp - 2) * 2 + (stores & 1)) * kStageOutBytes;
+                        if (h == 0 || sizeof(OT) == 4) {
+                            tma_store_wait_read<1>();  // by this thread: the store before the last one has read its buffer
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int j = 0; j < CHUNKS; ++j) {
+                            const int chunk = (sizeof(OT) == 4 ? 0 : CHUNKS * h) + j;
+                            *reinterpret_cast<uint4 *>(buf + lane * 128 + ((chunk ^ (lane & 7)) << 4)) =
+                                reinterpret_cast<const uint4 *>(o)[j];
+                        }
+                        if (h == HALVES - 1 || sizeof(OT) == 4) {
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            const int col = un.col0 + (sizeof(OT) == 4 ? c : c0);
+                            const int row_w = un.row0 + (int)rank * kRowTile + quad * 32;
+                            if (lane == 0) {
+                                if (row_w < p.rows && col < p.cols)
+                                    tma_store_3d(&tmOut, buf, col, row_w, un.split);
+                                tma_store_commit();
+                            }
+                            ++stores;
+                        }
+                    }
+                }
             }
             if (++acc == 2) {
                 acc = 0;
                 acc_phase ^= 1u;
             }
         }
+        if (!SWAP) tma_store_wait_read<0>();  // the buffers go with the CTA
     } else {
+        // ---------------------------------------------------------------- scales (both CTAs)
         int slot = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-            int m_blk, n_blk;
-            tile_coords(p, u, m_blk, n_blk);
-            for (int g = 0; 4 * g < p.nkb; ++g) {
-                const uint4 a = scale_words(p.a_scales, p.a_scale_pitch, p.a_shift, m_blk * kTile, p.M, g, lane);
-                const uint4 b = scale_words(p.b_scales, p.b_scale_pitch, p.b_shift, n_blk * kTile, p.N, g, lane);
+        for (int u = first_unit; ok && u < units; u += step_units) {
+            const Unit un = unit_of<S>(p, u);
+            for (int g = un.kb0 / 4; 4 * g < un.kb1; ++g) {
+                uint4 w[1 + S::COL_WORDS / 4];
+                w[0] = scale_words(p.r_scales, p.r_pitch, p.r_shift, un.row0 + (int)rank * kRowTile, p.rows, g, lane);
+#pragma unroll
+                for (int i = 0; i < S::COL_WORDS / 4; ++i)
+                    w[1 + i] = scale_words(p.c_scales, p.c_pitch, p.c_shift, un.col0 + 128 * i, p.cols, g, lane);
                 if (!(ok = wait(&sh->scale_empty[slot], phase ^ 1u))) break;
-                uint8_t *dst = sScale + slot * 1024 + lane * 16;
-                *reinterpret_cast<uint4 *>(dst) = a;
-                *reinterpret_cast<uint4 *>(dst + 512) = b;
+                uint8_t *dst = sScale + slot * S::SLOT_BYTES + lane * 16;
+#pragma unroll
+                for (int i = 0; i < 1 + S::COL_WORDS / 4; ++i) *reinterpret_cast<uint4 *>(dst + 512 * i) = w[i];
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->scale_full[slot]);
+                if (lane == 0) arrive_leader(&sh->scale_full[slot]);
                 if (++slot == kScaleSlots) {
                     slot = 0;
                     phase ^= 1u;
@@ -291,22 +458,121 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();  // the leader's MMAs no longer read this CTA's shared memory
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, kTmemCols);
+        if (PAIR)
+            tmem_dealloc_pair(tmem, kTmemCols);
+        else
+            tmem_dealloc(tmem, kTmemCols);
     }
 }
 
+// out = act(sum of the splits' partial sums, in order, + bias): four columns a thread.
 template <typename OT>
-int launch(const CUtensorMap &tmA, const CUtensorMap &tmB, const GemmParams &p, cudaStream_t stream) {
-    auto kern = block_gemm_kernel<OT>;
-    const size_t smem = 1024 + 2 * kStages * kTileBytes + kScaleSlots * 1024 + sizeof(Shared);
+__global__ void __launch_bounds__(256) join_splits_kernel(const float *__restrict__ part, int64_t split_stride,
+                                                          int64_t pitch, int splits, int M, int N,
+                                                          const float *__restrict__ bias,
+                                                          const float *__restrict__ thr, int activation,
+                                                          OT *__restrict__ out, int64_t out_pitch) {
+    const int n = (int)(blockIdx.x * blockDim.x + threadIdx.x) * 4;
+    if (n >= N) return;
+    for (int m = blockIdx.y; m < M; m += gridDim.y) {
+        const float *src = part + (int64_t)m * pitch + n;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int z = 0; z < splits; ++z) {
+            const float4 v = __ldg(reinterpret_cast<const float4 *>(src + z * split_stride));
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+        }
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < N)
+                out[(int64_t)m * out_pitch + n + j] = from_f32<OT>(
+                    activate(v[j] + (bias ? __ldg(bias + n + j) : 0.f), thr ? __ldg(thr + n + j) : 0.f, activation));
+    }
+}
+
+// ------------------------------------------------------------------------------- host side
+
+template <typename OT, typename S, bool SWAP>
+int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tmOut, const GemmParams &p,
+           cudaStream_t stream) {
+    auto kern = block_gemm_kernel<OT, S, SWAP>;
+    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + (SWAP ? 0 : 8 * kStageOutBytes) +
+                            kScaleSlots * S::SLOT_BYTES + sizeof(Shared);
+    static_assert(smem <= 232448, "shared memory per block");
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(block_gemm)");
-    kern<<<std::min(p.m_tiles * p.n_tiles, num_sms()), kThreads, smem, stream>>>(tmA, tmB, p);
+    const int units = p.row_tiles * p.col_tiles * p.splits;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    if (S::PAIR) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+        cfg.gridDim = dim3(2 * std::max(1, num_sms() / 2));
+        cfg.gridDim = dim3(2 * std::min(units, pair_slots(reinterpret_cast<const void *>(kern), cfg)));
+    } else {
+        cfg.gridDim = dim3(std::min(units, num_sms()));
+    }
+    e = cudaLaunchKernelEx(&cfg, kern, tmR, tmC, tmOut, p);
+    if (e != cudaSuccess) return check_cuda(e, "block_gemm launch");
     return check_cuda(cudaGetLastError(), "block_gemm launch");
 }
+
+using Pair = Shape<true, 256, 5>;
+using PairSwapped = Shape<true, 256, 6>;
+using One32 = Shape<false, 32, 10>;
+using One64 = Shape<false, 64, 8>;
+using One128 = Shape<false, 128, 6>;
+
+// What a call does, from its sizes alone.
+struct Plan {
+    bool pair, swap;
+    int cols;    // columns of a tile
+    int splits;  // ranges of K
+};
+
+int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+Plan make_plan(int64_t M, int64_t N, int64_t K, bool tma_out, int out_dtype) {
+    Plan pl{};
+    const int sms = num_sms();
+    const int groups = cdiv(K, 4 * kKBytes);
+    // Either kernel is paced by its operand loads, 32 KB per K block and CTA where the tile has 128 or
+    // 256 columns and less for narrow ones; a pair's tile is twice the work per CTA.
+    const int cols = M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const int64_t one_tiles = (int64_t)cdiv(N, 128) * cdiv(M, cols), pair_tiles = (int64_t)cdiv(N, 256) * cdiv(M, 256);
+    const int64_t one_cost = cdiv(one_tiles, sms) * (int64_t)(128 + cols), pair_cost = cdiv(pair_tiles, sms / 2) * 256;
+    pl.pair = M > 128 && pair_cost < one_cost;
+    pl.swap = !pl.pair || !tma_out;
+    pl.cols = pl.pair ? 256 : cols;
+    const int64_t tiles = pl.pair ? pair_tiles : one_tiles;
+    const int slots = pl.pair ? sms / 2 : sms;
+    // Few tiles: K is split among the idle SMs, 512 elements at least to each, and the partial sums joined.
+    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(groups, slots / tiles));
+    // The tensor cores round each addition toward zero, a bias that grows with the number of additions
+    // (measured against 64 bits: 9e-7 of the result at K = 8192, 1.2e-5 at 65536), far below a 16-bit
+    // output's rounding but not an fp32 one's: those sum ranges of at most 8192, joined in fp32.
+    if (out_dtype == SF_F32) pl.splits = std::max(pl.splits, cdiv(K, 8192));
+    // whole ranges: no split without a group
+    pl.splits = cdiv(groups, cdiv(groups, pl.splits));
+    return pl;
+}
+
+int64_t partial_pitch(int64_t N) { return (N + 3) / 4 * 4; }
 
 int check_product(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out) {
     int st = check_blocks(a, "a");
@@ -322,7 +588,24 @@ int check_product(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out) 
     // int coordinates, up to a tile past the end
     constexpr int64_t most = INT32_MAX - 4096;
     if (a->rows > most || b->rows > most || a->cols > most) return set_error(SF_ERR_UNSUPPORTED, "extent too large");
+    if ((int64_t)cdiv(a->rows, 32) * cdiv(b->rows, 128) > INT32_MAX / 512)
+        return set_error(SF_ERR_UNSUPPORTED, "too many output tiles");
     return SF_OK;
+}
+
+// Rows that TMA can write: 16-byte aligned base and pitch.
+bool tma_rows(const sf_matrix &out) {
+    return reinterpret_cast<uintptr_t>(out.data) % 16 == 0 && out.stride_row >= out.cols &&
+           (out.stride_row * (int64_t)dtype_size(out.dtype)) % 16 == 0;
+}
+
+template <typename OT>
+int run_plan(const Plan &pl, const CUtensorMap &r, const CUtensorMap &c, const CUtensorMap &o, const GemmParams &p,
+             cudaStream_t s) {
+    if (pl.pair) return pl.swap ? launch<OT, PairSwapped, true>(r, c, o, p, s) : launch<OT, Pair, false>(r, c, o, p, s);
+    if (pl.cols == 32) return launch<OT, One32, true>(r, c, o, p, s);
+    if (pl.cols == 64) return launch<OT, One64, true>(r, c, o, p, s);
+    return launch<OT, One128, true>(r, c, o, p, s);
 }
 
 }  // namespace
@@ -338,54 +621,94 @@ int sf_block_matmul_workspace(const sf_blocks *a, const sf_blocks *b, const sf_m
     if (st) return st;
     if (!bytes) return set_error(SF_ERR_INVALID, "bytes is NULL");
     *bytes = 0;
+    if (out->rows == 0 || out->cols == 0) return SF_OK;
+    const Plan pl = make_plan(a->rows, b->rows, a->cols, tma_rows(*out), out->dtype);
+    if (pl.splits > 1) *bytes = (size_t)pl.splits * out->rows * partial_pitch(out->cols) * sizeof(float);
     return SF_OK;
 }
 
 int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, const float *threshold, int activation,
                     const sf_matrix *out, void *workspace, size_t workspace_bytes, sf_stream stream) {
-    int st = check_product(a, b, out);
+    size_t need = 0;
+    int st = sf_block_matmul_workspace(a, b, out, &need);
     if (st) return st;
     if (activation != -1 && activation != SF_ACT_RELU && activation != SF_ACT_JUMPRELU)
         return set_error(SF_ERR_INVALID, "unknown activation %d", activation);
     if (activation == SF_ACT_JUMPRELU && !threshold) return set_error(SF_ERR_INVALID, "jumprelu needs a threshold");
     if (out->rows == 0 || out->cols == 0) return SF_OK;
-    (void)workspace;
-    (void)workspace_bytes;
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+        return set_error(SF_ERR_WORKSPACE, "16-byte aligned workspace of %zu bytes needed", need);
+    const int M = (int)a->rows, N = (int)b->rows;
+    const Plan pl = make_plan(M, N, a->cols, tma_rows(*out), out->dtype);
+    // Partial sums go to the workspace in fp32, without bias or activation, and are joined after.
+    const bool partial = pl.splits > 1;
+    sf_matrix dst = *out;
+    if (partial) {
+        dst.data = workspace;
+        dst.dtype = SF_F32;
+        dst.stride_row = partial_pitch(N);
+    }
+    const sf_blocks *R = pl.swap ? b : a, *C = pl.swap ? a : b;
+    const int row_tile = pl.pair ? 256 : 128;
     GemmParams p{};
-    p.M = (int)a->rows;
-    p.N = (int)b->rows;
-    p.nkb = (int)((a->cols + kKBytes - 1) / kKBytes);
-    p.m_tiles = (p.M + kTile - 1) / kTile;
-    p.n_tiles = (p.N + kTile - 1) / kTile;
-    if ((int64_t)p.m_tiles * p.n_tiles > INT32_MAX / 2) return set_error(SF_ERR_UNSUPPORTED, "too many output tiles");
-    // A group of m-tiles runs side by side over each n-tile: b is read from HBM once per group, while
-    // the group's 32 MB of a stay in L2.
-    p.group_m = (int)std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, (int64_t(32) << 20) / (kTile * a->cols)));
-    p.a_scales = static_cast<const uint8_t *>(a->scales);
-    p.b_scales = static_cast<const uint8_t *>(b->scales);
-    p.a_scale_pitch = a->scale_pitch;
-    p.b_scale_pitch = b->scale_pitch;
-    p.a_shift = a->tile ? 7 : 0;
-    p.b_shift = b->tile ? 7 : 0;
-    p.bias = bias;
-    p.thr = activation == SF_ACT_JUMPRELU ? threshold : nullptr;
-    p.activation = activation;
-    p.out = const_cast<void *>(out->data);
-    p.out_pitch = out->stride_row;
-    p.out_vec = (reinterpret_cast<uintptr_t>(out->data) % 16 == 0 &&
-                 (out->stride_row * (int64_t)dtype_size(out->dtype)) % 16 == 0)
-                    ? 1
-                    : 0;
+    p.rows = (int)R->rows;
+    p.cols = (int)C->rows;
+    p.nkb = cdiv(a->cols, kKBytes);
+    p.groups = cdiv(p.nkb, 4);
+    p.splits = pl.splits;
+    p.split_groups = cdiv(p.groups, pl.splits);
+    p.row_tiles = cdiv(p.rows, row_tile);
+    p.col_tiles = cdiv(p.cols, pl.cols);
+    // A group of row tiles runs side by side over each column tile: the columns' operand is read from HBM
+    // once per group, while the group's 32 MB stay in L2.
+    p.group_rows = (int)std::max<int64_t>(1, std::min<int64_t>(p.row_tiles, (int64_t(32) << 20) / (row_tile * a->cols)));
+    p.r_scales = static_cast<const uint8_t *>(R->scales);
+    p.c_scales = static_cast<const uint8_t *>(C->scales);
+    p.r_pitch = R->scale_pitch;
+    p.c_pitch = C->scale_pitch;
+    p.r_shift = R->tile ? 7 : 0;
+    p.c_shift = C->tile ? 7 : 0;
+    p.bias = partial ? nullptr : bias;
+    p.thr = partial || activation != SF_ACT_JUMPRELU ? nullptr : threshold;
+    p.activation = partial ? -1 : activation;
+    p.out = const_cast<void *>(dst.data);
+    p.out_pitch = dst.stride_row;
+    p.out_split = (int64_t)M * dst.stride_row;
     p.err = device_error_word();
-    CUtensorMap tmA, tmB;
-    if ((st = make_map_e4m3(&tmA, a->data, (uint64_t)a->cols, (uint64_t)a->rows, (uint64_t)a->data_pitch, kTile)))
+    CUtensorMap tmR, tmC, tmOut = {};
+    if ((st = make_map_e4m3(&tmR, R->data, (uint64_t)R->cols, (uint64_t)R->rows, (uint64_t)R->data_pitch, kRowTile)))
         return st;
-    if ((st = make_map_e4m3(&tmB, b->data, (uint64_t)b->cols, (uint64_t)b->rows, (uint64_t)b->data_pitch, kTile)))
+    if ((st = make_map_e4m3(&tmC, C->data, (uint64_t)C->cols, (uint64_t)C->rows, (uint64_t)C->data_pitch,
+                            pl.pair ? 128 : pl.cols)))
+        return st;
+    const int64_t es = (int64_t)dtype_size(dst.dtype);
+    if (!pl.swap &&
+        (st = make_map_out(&tmOut, dst.data, dst.dtype, (uint64_t)N, (uint64_t)M, (uint64_t)pl.splits,
+                           (uint64_t)(dst.stride_row * es), (uint64_t)(p.out_split * es))))
         return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (out->dtype == SF_BF16) return launch<__nv_bfloat16>(tmA, tmB, p, s);
-    if (out->dtype == SF_F16) return launch<__half>(tmA, tmB, p, s);
-    return launch<float>(tmA, tmB, p, s);
+    if (dst.dtype == SF_BF16)
+        st = run_plan<__nv_bfloat16>(pl, tmR, tmC, tmOut, p, s);
+    else if (dst.dtype == SF_F16)
+        st = run_plan<__half>(pl, tmR, tmC, tmOut, p, s);
+    else
+        st = run_plan<float>(pl, tmR, tmC, tmOut, p, s);
+    if (st || !partial) return st;
+    const dim3 grid(cdiv(N, 1024), std::min(M, 65535));
+    const float *part = static_cast<const float *>(workspace);
+    const float *thr = activation == SF_ACT_JUMPRELU ? threshold : nullptr;
+    void *o = const_cast<void *>(out->data);
+#define SF_JOIN(T)                                                                                                 \
+    join_splits_kernel<T><<<grid, 256, 0, s>>>(part, p.out_split, p.out_pitch, pl.splits, M, N, bias, thr, activation, \
+                                               static_cast<T *>(o), out->stride_row)
+    if (out->dtype == SF_BF16)
+        SF_JOIN(__nv_bfloat16);
+    else if (out->dtype == SF_F16)
+        SF_JOIN(__half);
+    else
+        SF_JOIN(float);
+#undef SF_JOIN
+    return check_cuda(cudaGetLastError(), "join_splits launch");
 }
 
 }  // extern "C"
