@@ -22,6 +22,7 @@
 // suits outputs whose rows TMA cannot address, and few rows of `a` make a narrow tile (COLS = 32) beside
 // 128 rows of weights.
 #include <algorithm>
+#include <type_traits>
 
 #include "sf_common.cuh"
 #include "sf_internal.h"
@@ -34,8 +35,19 @@ constexpr int kKBytes = 128;                   // elements (bytes) of K per stag
 constexpr int kScaleSlots = 3;                 // scale words of 512 elements of K each
 constexpr int kThreads = 224;
 constexpr int kTmemCols = 512;
+constexpr int kPairCols = 256;                 // columns of a pair's tile
 constexpr int kRowTile = 128;                  // rows (TMEM lanes) per CTA
-constexpr int kStageOutBytes = 4096;           // 32 output rows x 128 bytes of one epilogue warp
+
+// Division of n < 2^31 by a divisor d >= 1 known on the host: n / d = high 64 bits of n * (floor(2^64 / d) + 1)
+// (for d = 1 that does not fit 64 bits). A plain division is a chain of some 150 clocks,
+// and a tile's coordinates take four.
+struct Divisor {
+    unsigned long long magic;
+    int d;
+    __device__ __forceinline__ int div(int n) const {
+        return d == 1 ? n : (int)__umul64hi((unsigned long long)n, magic);
+    }
+};
 
 struct GemmParams {
     int rows, cols;            // of the tile grid: a's and b's, or b's and a's with SWAP
@@ -43,6 +55,7 @@ struct GemmParams {
     int splits, split_groups;  // ranges of K: split z takes groups [z split_groups, (z + 1) split_groups)
     int row_tiles, col_tiles;
     int group_rows;            // row tiles that run side by side over each column tile
+    Divisor by_tiles, by_group, by_rows, by_last_rows;  // tiles, tiles of a group, rows of a group, of the last
     const uint8_t *r_scales, *c_scales;  // of the rows' and the columns' operand
     int64_t r_pitch, c_pitch;
     int r_shift, c_shift;      // log2 of the rows a scale row serves: 0 row blocks, 7 tiles
@@ -63,11 +76,12 @@ struct Shape {
     static constexpr int COLS_HERE = PAIR ? COLS / 2 : COLS;    // rows of the columns' operand loaded per CTA
     static constexpr int STAGES = STAGES_;
     static constexpr int R_BYTES = kRowTile * kKBytes, C_BYTES = COLS_HERE * kKBytes;
-    static constexpr int COL_WORDS = COLS <= 128 ? 4 : COLS / 32;  // TMEM columns of the columns' scales
+    static constexpr int COL_WORDS = COLS <= 128 ? 4 : 8;  // TMEM columns of the columns' scales
     static constexpr int SLOT_COLS = 4 + COL_WORDS;
     static constexpr int SLOT_BYTES = 512 + COL_WORDS / 4 * 512;
-    // Two accumulators and the scales in 512 columns: at 256 columns the accumulators overlap by 40.
+    // Two accumulators and the scales in 512 columns of TMEM: at 256 columns the accumulators overlap by 40.
     static constexpr int ACC1 = COLS == 256 ? 216 : COLS;
+    static constexpr bool OVERLAP = ACC1 < COLS;
     static constexpr int SCALE_COL = ACC1 + COLS;
     static_assert(SCALE_COL + kScaleSlots * SLOT_COLS <= kTmemCols, "TMEM columns");
 };
@@ -90,16 +104,16 @@ struct Unit {
 template <typename S>
 __device__ __forceinline__ Unit unit_of(const GemmParams &p, int u) {
     Unit r;
-    const int tiles = p.row_tiles * p.col_tiles;
-    r.split = u / tiles;
-    u -= r.split * tiles;
-    const int per_group = p.group_rows * p.col_tiles;
-    const int g = u / per_group;
+    r.split = p.by_tiles.div(u);
+    u -= r.split * p.by_tiles.d;
+    const int g = p.by_group.div(u);
     const int first = g * p.group_rows;
-    const int gm = min(p.row_tiles - first, p.group_rows);
-    const int local = u - g * per_group;
-    r.row0 = (first + local % gm) * S::ROWS;
-    r.col0 = local / gm * S::COLS;
+    const bool last = p.row_tiles - first < p.group_rows;
+    const Divisor by = last ? p.by_last_rows : p.by_rows;
+    const int local = u - g * p.by_group.d;
+    const int col = by.div(local);
+    r.row0 = (first + local - col * by.d) * S::ROWS;
+    r.col0 = col * S::COLS;
     r.kb0 = 4 * r.split * p.split_groups;
     r.kb1 = min(p.nkb, r.kb0 + 4 * p.split_groups);
     return r;
@@ -118,10 +132,33 @@ __device__ __forceinline__ uint4 scale_words(const uint8_t *s, int64_t pitch, in
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ float activate(float v, float t, int activation) {
-    if (activation == SF_ACT_RELU) return v < 0.f ? 0.f : v;  // fmaxf would turn a NaN into 0
-    if (activation == SF_ACT_JUMPRELU) return v > t && v > 0.f ? v : 0.f;
-    return v;
+// max(v, floor) that keeps a NaN (fmaxf would drop it): ReLU with floor 0, nothing with floor -inf.
+__device__ __forceinline__ float at_least(float v, float floor) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(floor));
+    return r;
+}
+__device__ __forceinline__ float jump(float v, float t) { return v > t && v > 0.f ? v : 0.f; }
+__device__ __forceinline__ float floor_of(int activation) {
+    return activation == SF_ACT_RELU ? 0.f : __int_as_float(0xff800000);
+}
+
+// Bias and activation of 32 columns. The activation is uniform: one test per 32 columns, none per element
+// (with a test per element this loop took 1350 clocks, four times the rest of the epilogue).
+__device__ __forceinline__ void finish_columns(const uint32_t (&r)[32], const float *bias, const float *thr,
+                                               float floor, float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 b = *reinterpret_cast<const float4 *>(bias + j);
+        v[j] = at_least(__uint_as_float(r[j]) + b.x, floor);
+        v[j + 1] = at_least(__uint_as_float(r[j + 1]) + b.y, floor);
+        v[j + 2] = at_least(__uint_as_float(r[j + 2]) + b.z, floor);
+        v[j + 3] = at_least(__uint_as_float(r[j + 3]) + b.w, floor);
+    }
+    if (thr) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = jump(v[j], thr[j]);
+    }
 }
 
 template <typename OT, typename S, bool SWAP>
@@ -133,8 +170,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sR = smem;
     uint8_t *sC = sR + S::STAGES * S::R_BYTES;
+    constexpr int OUT_BYTES = 32 * 32 * sizeof(OT);
     uint8_t *sOut = sC + S::STAGES * S::C_BYTES;  // 4 warps x 2 buffers (not with SWAP)
-    uint8_t *sScale = sOut + (SWAP ? 0 : 8 * kStageOutBytes);
+    uint8_t *sScale = sOut + (SWAP ? 0 : 8 * OUT_BYTES);
     Shared *sh = reinterpret_cast<Shared *>(sScale + kScaleSlots * S::SLOT_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -265,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Unit un = unit_of<S>(p, u);
                 // Accumulators that overlap: the previous tile's epilogue must have read the columns that
                 // this tile's shares with it (and so has finished the tile before that).
-                if (S::ACC1 < S::COLS) {
+                if (S::OVERLAP) {
                     if (!first_tile && !(ok = wait(&sh->tmem_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1u))) break;
                     first_tile = false;
                 } else if (!(ok = wait(&sh->tmem_empty[acc], acc_phase ^ 1u))) {
@@ -334,47 +372,60 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---------------------------------------------------------------- epilogue
         const int et = threadIdx.x - 64;
         const int quad = warp & 3;
-        constexpr int STEP = 64;  // columns loaded at a time
-        constexpr int STEPS = (S::COLS + STEP - 1) / STEP;
-        constexpr int HALVES = S::COLS < STEP ? 1 : 2;
+        constexpr int STEP = S::COLS < 64 ? S::COLS : 64;  // columns loaded at a time
+        constexpr int STEPS = S::COLS / STEP;
+        const float floor = floor_of(p.activation);
         int acc = 0;
         uint32_t acc_phase = 0;
         int stores = 0;
+        // This thread's bias and threshold of the coming tile, loaded a tile ahead: its row's with SWAP, else
+        // those of columns et and et + 128, for shared memory.
+        constexpr int OWN = SWAP ? 1 : S::COLS / 128;
+        float next_bias[OWN], next_thr[OWN];
+        auto load_vectors = [&](int u) {
+            const Unit un = unit_of<S>(p, min(u, units - 1));
+#pragma unroll
+            for (int j = 0; j < OWN; ++j) {
+                const int at = SWAP ? un.row0 + (int)rank * kRowTile + quad * 32 + lane : un.col0 + et + 128 * j;
+                const bool have = at < (SWAP ? p.rows : p.cols);
+                next_bias[j] = p.bias && have ? __ldg(p.bias + at) : 0.f;
+                next_thr[j] = p.thr && have ? __ldg(p.thr + at) : 0.f;
+            }
+        };
+        load_vectors(first_unit);
         for (int u = first_unit; u < units; u += step_units) {
             const Unit un = unit_of<S>(p, u);
             const int row = un.row0 + (int)rank * kRowTile + quad * 32 + lane;
-            float row_bias = 0.f, row_thr = 0.f;
-            if (SWAP) {
-                if (p.bias && row < p.rows) row_bias = __ldg(p.bias + row);
-                if (p.thr && row < p.rows) row_thr = __ldg(p.thr + row);
-            } else {
-                for (int j = et; j < S::COLS; j += 128) {
-                    const int col = un.col0 + j;
-                    sh->bias[acc][j] = p.bias && col < p.cols ? __ldg(p.bias + col) : 0.f;
-                    sh->thr[acc][j] = p.thr && col < p.cols ? __ldg(p.thr + col) : 0.f;
+            const float row_bias = next_bias[0], row_thr = next_thr[0];
+            if (!SWAP) {
+#pragma unroll
+                for (int j = 0; j < OWN; ++j) {
+                    sh->bias[acc][et + 128 * j] = next_bias[j];
+                    sh->thr[acc][et + 128 * j] = next_thr[j];
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
             }
+            load_vectors(u + step_units);
             if (!wait(&sh->tmem_full[acc], acc_phase)) break;
             tc_fence_after();
             const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1;
             // Overlapping accumulators: the shared columns (the first's last 40, the second's first 40) are
             // read first and released to the next tile's MMAs.
-            const int first = S::ACC1 < S::COLS && acc == 0 ? STEPS - 1 : 0;
+            const int first = S::OVERLAP && acc == 0 ? STEPS - 1 : 0;
 #pragma unroll 1
             for (int i = 0; i < STEPS; ++i) {
                 const int c0 = (first + i) % STEPS * STEP;
-                uint32_t r[HALVES][32];
+                uint32_t r[STEP / 32][32];
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
+                for (int h = 0; h < STEP / 32; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
                 tmem_ld_wait();
-                if (i == (S::ACC1 < S::COLS ? 0 : STEPS - 1)) {
+                if (i == (S::OVERLAP ? 0 : STEPS - 1)) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_leader(&sh->tmem_empty[acc]);
                 }
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) {
+                for (int h = 0; h < STEP / 32; ++h) {
                     const int c = c0 + 32 * h;
                     if constexpr (SWAP) {
                         if (row < p.rows) {
@@ -382,43 +433,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                                       (int64_t)(un.col0 + c) * p.out_pitch + row;
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
-                                if (un.col0 + c + j < p.cols)
-                                    dst[j * p.out_pitch] = from_f32<OT>(
-                                        activate(__uint_as_float(r[h][j]) + row_bias, row_thr, p.activation));
+                                float v = at_least(__uint_as_float(r[h][j]) + row_bias, floor);
+                                if (p.thr) v = jump(v, row_thr);
+                                if (un.col0 + c + j < p.cols) dst[j * p.out_pitch] = from_f32<OT>(v);
                             }
                         }
                     } else {
+                        float v[32];
+                        finish_columns(r[h], sh->bias[acc] + c, p.thr ? sh->thr[acc] + c : nullptr, floor, v);
                         alignas(16) OT o[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            o[j] = from_f32<OT>(activate(__uint_as_float(r[h][j]) + sh->bias[acc][c + j],
-                                                         sh->thr[acc][c + j], p.activation));
-                        // 32 rows x 128 bytes, 16-byte chunk j of row r at chunk j ^ (r % 8): 32 columns of fp32,
-                        // or both halves of 16-bit outputs
+                        for (int j = 0; j < 32; ++j) o[j] = from_f32<OT>(v[j]);
+                        uint8_t *buf = sOut + ((warp - 2) * 2 + (stores & 1)) * OUT_BYTES;
+                        tma_store_wait_read<1>();  // the store before the last one has read its buffer
+                        __syncwarp();
+                        // 32 rows of 32 columns, 16-byte chunks swizzled as the tensor map says: 128-byte rows of fp32
+                        // (chunk ^ row % 8), 64-byte rows of 16-bit outputs (chunk ^ row / 2 % 4)
                         constexpr int CHUNKS = 2 * sizeof(OT);
-                        uint8_t *buf = sOut + ((warp - 2) * 2 + (stores & 1)) * kStageOutBytes;
-                        if (h == 0 || sizeof(OT) == 4) {
-                            tma_store_wait_read<1>();  // by this thread: the store before the last one has read its buffer
-                            __syncwarp();
-                        }
+                        const int swz = sizeof(OT) == 4 ? lane & 7 : (lane >> 1) & 3;
 #pragma unroll
-                        for (int j = 0; j < CHUNKS; ++j) {
-                            const int chunk = (sizeof(OT) == 4 ? 0 : CHUNKS * h) + j;
-                            *reinterpret_cast<uint4 *>(buf + lane * 128 + ((chunk ^ (lane & 7)) << 4)) =
+                        for (int j = 0; j < CHUNKS; ++j)
+                            *reinterpret_cast<uint4 *>(buf + lane * (16 * CHUNKS) + ((j ^ swz) << 4)) =
                                 reinterpret_cast<const uint4 *>(o)[j];
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        const int row_w = un.row0 + (int)rank * kRowTile + quad * 32;
+                        if (lane == 0) {
+                            if (row_w < p.rows && un.col0 + c < p.cols)
+                                tma_store_3d(&tmOut, buf, un.col0 + c, row_w, un.split);
+                            tma_store_commit();
                         }
-                        if (h == HALVES - 1 || sizeof(OT) == 4) {
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            const int col = un.col0 + (sizeof(OT) == 4 ? c : c0);
-                            const int row_w = un.row0 + (int)rank * kRowTile + quad * 32;
-                            if (lane == 0) {
-                                if (row_w < p.rows && col < p.cols)
-                                    tma_store_3d(&tmOut, buf, col, row_w, un.split);
-                                tma_store_commit();
-                            }
-                            ++stores;
-                        }
+                        ++stores;
                     }
                 }
             }
@@ -491,10 +536,12 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const float *__restric
         }
         const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (n + j < N)
-                out[(int64_t)m * out_pitch + n + j] = from_f32<OT>(
-                    activate(v[j] + (bias ? __ldg(bias + n + j) : 0.f), thr ? __ldg(thr + n + j) : 0.f, activation));
+        for (int j = 0; j < 4; ++j) {
+            if (n + j >= N) break;
+            float t = at_least(v[j] + (bias ? __ldg(bias + n + j) : 0.f), floor_of(activation));
+            if (thr) t = jump(t, __ldg(thr + n + j));
+            out[(int64_t)m * out_pitch + n + j] = from_f32<OT>(t);
+        }
     }
 }
 
@@ -504,7 +551,7 @@ template <typename OT, typename S, bool SWAP>
 int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tmOut, const GemmParams &p,
            cudaStream_t stream) {
     auto kern = block_gemm_kernel<OT, S, SWAP>;
-    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + (SWAP ? 0 : 8 * kStageOutBytes) +
+    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + (SWAP ? 0 : 8 * 32 * 32 * sizeof(OT)) +
                             kScaleSlots * S::SLOT_BYTES + sizeof(Shared);
     static_assert(smem <= 232448, "shared memory per block");
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -532,8 +579,8 @@ int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tm
     return check_cuda(cudaGetLastError(), "block_gemm launch");
 }
 
-using Pair = Shape<true, 256, 5>;
-using PairSwapped = Shape<true, 256, 6>;
+using Pair16 = Shape<true, kPairCols, 6>;  // 16-bit outputs, or SWAP
+using Pair32 = Shape<true, kPairCols, 5>;  // fp32 outputs: larger store buffers
 using One32 = Shape<false, 32, 10>;
 using One64 = Shape<false, 64, 8>;
 using One128 = Shape<false, 128, 6>;
@@ -551,14 +598,15 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool tma_out, int out_dtype) {
     Plan pl{};
     const int sms = num_sms();
     const int groups = cdiv(K, 4 * kKBytes);
-    // Either kernel is paced by its operand loads, 32 KB per K block and CTA where the tile has 128 or
-    // 256 columns and less for narrow ones; a pair's tile is twice the work per CTA.
+    // Either kernel is paced by its operand loads, 128 + columns rows per K block and
+    // CTA (a pair's CTA loads half of its columns), and a pair's tile is twice the work per CTA.
     const int cols = M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t one_tiles = (int64_t)cdiv(N, 128) * cdiv(M, cols), pair_tiles = (int64_t)cdiv(N, 256) * cdiv(M, 256);
+    const int64_t one_tiles = (int64_t)cdiv(N, 128) * cdiv(M, cols);
+    const int64_t pair_tiles = tma_out ? (int64_t)cdiv(N, kPairCols) * cdiv(M, 256) : (int64_t)cdiv(N, 256) * cdiv(M, kPairCols);
     const int64_t one_cost = cdiv(one_tiles, sms) * (int64_t)(128 + cols), pair_cost = cdiv(pair_tiles, sms / 2) * 256;
     pl.pair = M > 128 && pair_cost < one_cost;
     pl.swap = !pl.pair || !tma_out;
-    pl.cols = pl.pair ? 256 : cols;
+    pl.cols = pl.pair ? kPairCols : cols;
     const int64_t tiles = pl.pair ? pair_tiles : one_tiles;
     const int slots = pl.pair ? sms / 2 : sms;
     // Few tiles: K is split among the idle SMs, 512 elements at least to each, and the partial sums joined.
@@ -571,6 +619,8 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool tma_out, int out_dtype) {
     pl.splits = cdiv(groups, cdiv(groups, pl.splits));
     return pl;
 }
+
+Divisor divisor(int d) { return Divisor{~0ull / (unsigned)d + 1, d}; }
 
 int64_t partial_pitch(int64_t N) { return (N + 3) / 4 * 4; }
 
@@ -602,7 +652,8 @@ bool tma_rows(const sf_matrix &out) {
 template <typename OT>
 int run_plan(const Plan &pl, const CUtensorMap &r, const CUtensorMap &c, const CUtensorMap &o, const GemmParams &p,
              cudaStream_t s) {
-    if (pl.pair) return pl.swap ? launch<OT, PairSwapped, true>(r, c, o, p, s) : launch<OT, Pair, false>(r, c, o, p, s);
+    using Pair = std::conditional_t<sizeof(OT) == 4, Pair32, Pair16>;
+    if (pl.pair) return pl.swap ? launch<OT, Pair16, true>(r, c, o, p, s) : launch<OT, Pair, false>(r, c, o, p, s);
     if (pl.cols == 32) return launch<OT, One32, true>(r, c, o, p, s);
     if (pl.cols == 64) return launch<OT, One64, true>(r, c, o, p, s);
     return launch<OT, One128, true>(r, c, o, p, s);
@@ -640,6 +691,8 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
         return set_error(SF_ERR_WORKSPACE, "16-byte aligned workspace of %zu bytes needed", need);
     const int M = (int)a->rows, N = (int)b->rows;
     const Plan pl = make_plan(M, N, a->cols, tma_rows(*out), out->dtype);
+    if ((int64_t)cdiv(M, 32) * cdiv(N, 128) * pl.splits > INT32_MAX / 2)
+        return set_error(SF_ERR_UNSUPPORTED, "too many output tiles and ranges of K");
     // Partial sums go to the workspace in fp32, without bias or activation, and are joined after.
     const bool partial = pl.splits > 1;
     sf_matrix dst = *out;
@@ -662,6 +715,10 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     // A group of row tiles runs side by side over each column tile: the columns' operand is read from HBM
     // once per group, while the group's 32 MB stay in L2.
     p.group_rows = (int)std::max<int64_t>(1, std::min<int64_t>(p.row_tiles, (int64_t(32) << 20) / (row_tile * a->cols)));
+    p.by_tiles = divisor(p.row_tiles * p.col_tiles);
+    p.by_group = divisor(p.group_rows * p.col_tiles);
+    p.by_rows = divisor(p.group_rows);
+    p.by_last_rows = divisor(p.row_tiles % p.group_rows ? p.row_tiles % p.group_rows : p.group_rows);
     p.r_scales = static_cast<const uint8_t *>(R->scales);
     p.c_scales = static_cast<const uint8_t *>(C->scales);
     p.r_pitch = R->scale_pitch;
@@ -679,7 +736,7 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     if ((st = make_map_e4m3(&tmR, R->data, (uint64_t)R->cols, (uint64_t)R->rows, (uint64_t)R->data_pitch, kRowTile)))
         return st;
     if ((st = make_map_e4m3(&tmC, C->data, (uint64_t)C->cols, (uint64_t)C->rows, (uint64_t)C->data_pitch,
-                            pl.pair ? 128 : pl.cols)))
+                            pl.pair ? kPairCols / 2 : pl.cols)))
         return st;
     const int64_t es = (int64_t)dtype_size(dst.dtype);
     if (!pl.swap &&
