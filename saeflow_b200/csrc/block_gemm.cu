@@ -295,7 +295,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (the leader's)
-        if (leader && lane == 0) {
+        // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers, and
+        // one elected lane issues: with the loop inside a one-lane branch each instruction's operands were
+        // moved there one by one (some 140 clocks an MMA, more than a 256 x 256 x 32 one takes).
+        if (leader) {
+            const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t desc_r = smem_desc_sw128(smem_u32(sR), 16, 1024);
+            const uint64_t desc_c = smem_desc_sw128(smem_u32(sC), 16, 1024);
+            const uint64_t desc_s = smem_desc_rows16(smem_u32(sScale));
             int stage = 0, slot = 0, acc = 0;
             uint32_t phase = 0, slot_phase = 0, acc_phase = 0;
             bool ok = true, first_tile = true;
@@ -310,62 +317,69 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem + acc * S::ACC1;
-                uint32_t scales = 0;
-                for (int kb = un.kb0; kb < un.kb1; ++kb) {
-                    if ((kb & 3) == 0) {
-                        if (!(ok = wait_cluster(&sh->scale_full[slot], slot_phase))) break;
-                        tc_fence_after();
-                        scales = tmem + S::SCALE_COL + slot * S::SLOT_COLS;
-                        const uint32_t src = smem_u32(sScale + slot * S::SLOT_BYTES);
+                const uint32_t d = tmem_u + acc * S::ACC1;
+                for (int kb4 = un.kb0; ok && kb4 < un.kb1; kb4 += 4) {
+                    if (!(ok = wait_cluster(&sh->scale_full[slot], slot_phase))) break;
+                    tc_fence_after();
+                    const uint32_t scales = tmem_u + S::SCALE_COL + slot * S::SLOT_COLS;
+                    if (elect_one()) {
+                        const uint64_t src = desc_s + slot * (S::SLOT_BYTES >> 4);
 #pragma unroll
                         for (int i = 0; i < S::SLOT_COLS / 4; ++i) {
                             if (PAIR)
-                                tmem_copy_32x128b_pair(scales + 4 * i, smem_desc_rows16(src + 512 * i));
+                                tmem_copy_32x128b_pair(scales + 4 * i, src + 32 * i);
                             else
-                                tmem_copy_32x128b(scales + 4 * i, smem_desc_rows16(src + 512 * i));
+                                tmem_copy_32x128b(scales + 4 * i, src + 32 * i);
                         }
                     }
-                    if (!(ok = wait(&sh->full[stage], phase))) break;
-                    tc_fence_after();
-                    const uint32_t r = smem_u32(sR + stage * S::R_BYTES), c = smem_u32(sC + stage * S::C_BYTES);
-                    const uint32_t idesc = make_idesc_e4m3_scaled(S::ROWS, S::COLS, kb & 3);
+                    __syncwarp();
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        const uint64_t rd = smem_desc_sw128(r + ks * 32, 16, 1024);
-                        const uint64_t cd = smem_desc_sw128(c + ks * 32, 16, 1024);
-                        const uint32_t accumulate = (kb > un.kb0 || ks) ? 1u : 0u;
-                        if (PAIR)
-                            umma_e4m3_scaled_pair(d, rd, cd, idesc, scales, scales + 4, accumulate);
-                        else
-                            umma_e4m3_scaled(d, rd, cd, idesc, scales, scales + 4, accumulate);
-                    }
-                    commit(&sh->empty[stage]);
-                    if (++stage == S::STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                    // Released with the group's last MMA: a slot is filled again, in shared memory and
-                    // then in TMEM, only after the MMAs that read it.
-                    if ((kb & 3) == 3 || kb + 1 == un.kb1) {
-                        commit(&sh->scale_empty[slot]);
-                        if (++slot == kScaleSlots) {
-                            slot = 0;
-                            slot_phase ^= 1u;
+                    for (int j = 0; j < 4; ++j) {
+                        if (kb4 + j >= un.kb1) break;
+                        if (!(ok = wait(&sh->full[stage], phase))) break;
+                        tc_fence_after();
+                        const uint64_t rd = desc_r + stage * (S::R_BYTES >> 4), cd = desc_c + stage * (S::C_BYTES >> 4);
+                        constexpr uint32_t IDESC0 = make_idesc_e4m3_scaled(S::ROWS, S::COLS, 0);
+                        const uint32_t idesc = IDESC0 | (j << 4) | (j << 29);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) {
+                                const uint32_t accumulate = (kb4 > un.kb0 || j || ks) ? 1u : 0u;
+                                if (PAIR)
+                                    umma_e4m3_scaled_pair(d, rd + 2 * ks, cd + 2 * ks, idesc, scales, scales + 4,
+                                                          accumulate);
+                                else
+                                    umma_e4m3_scaled(d, rd + 2 * ks, cd + 2 * ks, idesc, scales, scales + 4, accumulate);
+                            }
+                            commit(&sh->empty[stage]);
+                            // Released with the group's last MMA: a slot is filled again, in shared memory and
+                            // then in TMEM, only after the MMAs that read it.
+                            if (j == 3 || kb4 + j + 1 == un.kb1) commit(&sh->scale_empty[slot]);
+                            if (kb4 + j + 1 == un.kb1) commit(&sh->tmem_full[acc]);
                         }
+                        __syncwarp();
+                        if (++stage == S::STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                    if (++slot == kScaleSlots) {
+                        slot = 0;
+                        slot_phase ^= 1u;
                     }
                 }
-                if (!ok) break;
-                commit(&sh->tmem_full[acc]);
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
             }
-            if (PAIR)
-                umma_commit_pair(map_to_rank(smem_u32(&sh->drain), 0));
-            else
-                umma_commit(&sh->drain);
+            if (elect_one()) {
+                if (PAIR)
+                    umma_commit_pair(map_to_rank(smem_u32(&sh->drain), 0));
+                else
+                    umma_commit(&sh->drain);
+            }
+            __syncwarp();
             mbar_wait_drain(&sh->drain, 0, p.err);
         }
     } else if (warp < 6) {
