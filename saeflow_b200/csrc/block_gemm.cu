@@ -8,11 +8,11 @@
 // the instruction descriptor says which byte of the word applies. Tiles (one scale per 128 x 128) are
 // the same words read once per 128 rows.
 //
-// Persistent kernel, one CTA per SM, warp-specialised (224 threads):
+// Persistent kernel, one CTA per SM, warp-specialised (352 threads):
 //   warp 0      TMA producer: 128-byte rows of both operands, SWIZZLE_128B, mbarrier ring
 //   warp 1      TMEM allocator and MMA issuer
-//   warps 2-5   epilogue: bias, activation, rounding, stores
-//   warp 6      scale words of both operands for 512 elements of K into shared memory, in the order that
+//   warps 2-9   epilogue: bias, activation, rounding, stores; two warps to 32 rows, half the columns each
+//   warp 10     scale words of both operands for 512 elements of K into shared memory, in the order that
 //               tcgen05.cp spreads over TMEM (row r at byte 16 (r % 32) + 4 (r / 32))
 //
 // Two sizes. PAIR: a CTA pair (cta_group::2) computes 256 x 256, each CTA loading 128 rows of either
@@ -33,7 +33,8 @@ namespace {
 
 constexpr int kKBytes = 128;                   // elements (bytes) of K per stage
 constexpr int kScaleSlots = 3;                 // scale words of 512 elements of K each
-constexpr int kThreads = 224;
+constexpr int kEpilogueWarps = 8;               // two for each quarter of the TMEM lanes
+constexpr int kThreads = 32 * (3 + kEpilogueWarps);
 constexpr int kTmemCols = 512;
 constexpr int kPairCols = 256;                 // columns of a pair's tile
 constexpr int kRowTile = 128;                  // rows (TMEM lanes) per CTA
@@ -54,6 +55,7 @@ struct GemmParams {
     int nkb, groups;           // K blocks of 128, and groups of four of them
     int splits, split_groups;  // ranges of K: split z takes groups [z split_groups, (z + 1) split_groups)
     int row_tiles, col_tiles;
+    int col_bytes;             // the columns' operand per CTA and stage, as its TMA box is cut
     int group_rows;            // row tiles that run side by side over each column tile
     Divisor by_tiles, by_group, by_rows, by_last_rows;  // tiles, tiles of a group, rows of a group, of the last
     const uint8_t *r_scales, *c_scales;  // of the rows' and the columns' operand
@@ -171,8 +173,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *sR = smem;
     uint8_t *sC = sR + S::STAGES * S::R_BYTES;
     constexpr int OUT_BYTES = 32 * 32 * sizeof(OT);
-    uint8_t *sOut = sC + S::STAGES * S::C_BYTES;  // 4 warps x 2 buffers (not with SWAP)
-    uint8_t *sScale = sOut + (SWAP ? 0 : 8 * OUT_BYTES);
+    uint8_t *sOut = sC + S::STAGES * S::C_BYTES;  // one buffer per epilogue warp (not with SWAP)
+    uint8_t *sScale = sOut + (SWAP ? 0 : kEpilogueWarps * OUT_BYTES);
     Shared *sh = reinterpret_cast<Shared *>(sScale + kScaleSlots * S::SLOT_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sh->tmem_full[b], 1);
-            mbar_init(&sh->tmem_empty[b], 4 * kCtas);  // leader's: one arrive per epilogue warp
+            mbar_init(&sh->tmem_empty[b], kEpilogueWarps * kCtas);  // leader's: one arrive per epilogue warp
         }
         mbar_init(&sh->drain, 1);
         sh->abort_flag = 0;
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int kb = un.kb0; kb < un.kb1; ++kb) {
                     if (!(ok = wait(&sh->empty[stage], phase ^ 1u))) break;
                     if (leader) {
-                        mbar_arrive_expect_tx(&sh->full[stage], kCtas * (S::R_BYTES + S::C_BYTES));
+                        mbar_arrive_expect_tx(&sh->full[stage], kCtas * (S::R_BYTES + p.col_bytes));
                         armed |= 1u << stage;
                         armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
                     }
@@ -382,62 +384,63 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             mbar_wait_drain(&sh->drain, 0, p.err);
         }
-    } else if (warp < 6) {
+    } else if (warp < 2 + kEpilogueWarps) {
         // ---------------------------------------------------------------- epilogue
         const int et = threadIdx.x - 64;
         const int quad = warp & 3;
-        constexpr int STEP = S::COLS < 64 ? S::COLS : 64;  // columns loaded at a time
-        constexpr int STEPS = S::COLS / STEP;
+        // This warp's columns: a half of the tile's, or the first warp all 32 of the narrowest.
+        constexpr int HALF = S::COLS < 64 ? S::COLS : S::COLS / 2;
+        constexpr int STEP = HALF < 64 ? HALF : 64;  // columns loaded at a time
+        constexpr int STEPS = HALF / STEP;
+        const int half = (warp - 2) >> 2;
+        const int my_steps = half * HALF < S::COLS ? STEPS : 0;
         const float floor = floor_of(p.activation);
         int acc = 0;
         uint32_t acc_phase = 0;
-        int stores = 0;
         // This thread's bias and threshold of the coming tile, loaded a tile ahead: its row's with SWAP, else
-        // those of columns et and et + 128, for shared memory.
-        constexpr int OWN = SWAP ? 1 : S::COLS / 128;
-        float next_bias[OWN], next_thr[OWN];
+        // column et's, for shared memory.
+        static_assert(SWAP || S::COLS == 32 * kEpilogueWarps, "a column to each epilogue thread");
+        float next_bias, next_thr;
         auto load_vectors = [&](int u) {
             const Unit un = unit_of<S>(p, min(u, units - 1));
-#pragma unroll
-            for (int j = 0; j < OWN; ++j) {
-                const int at = SWAP ? un.row0 + (int)rank * kRowTile + quad * 32 + lane : un.col0 + et + 128 * j;
-                const bool have = at < (SWAP ? p.rows : p.cols);
-                next_bias[j] = p.bias && have ? __ldg(p.bias + at) : 0.f;
-                next_thr[j] = p.thr && have ? __ldg(p.thr + at) : 0.f;
-            }
+            const int at = SWAP ? un.row0 + (int)rank * kRowTile + quad * 32 + lane : un.col0 + et;
+            const bool have = at < (SWAP ? p.rows : p.cols);
+            next_bias = p.bias && have ? __ldg(p.bias + at) : 0.f;
+            next_thr = p.thr && have ? __ldg(p.thr + at) : 0.f;
         };
         load_vectors(first_unit);
         for (int u = first_unit; u < units; u += step_units) {
             const Unit un = unit_of<S>(p, u);
             const int row = un.row0 + (int)rank * kRowTile + quad * 32 + lane;
-            const float row_bias = next_bias[0], row_thr = next_thr[0];
+            const float row_bias = next_bias, row_thr = next_thr;
             if (!SWAP) {
-#pragma unroll
-                for (int j = 0; j < OWN; ++j) {
-                    sh->bias[acc][et + 128 * j] = next_bias[j];
-                    sh->thr[acc][et + 128 * j] = next_thr[j];
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                sh->bias[acc][et] = next_bias;
+                sh->thr[acc][et] = next_thr;
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
             }
             load_vectors(u + step_units);
             if (!wait(&sh->tmem_full[acc], acc_phase)) break;
             tc_fence_after();
             const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1;
             // Overlapping accumulators: the shared columns (the first's last 40, the second's first 40) are
-            // read first and released to the next tile's MMAs.
+            // read first and released to the next tile's MMAs. A warp whose half has none of them releases at
+            // once: what it still had to read of the tile before, in the accumulator that those MMAs take, it has.
+            const bool shares = !S::OVERLAP || half == (acc ^ 1);
+            auto release = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&sh->tmem_empty[acc]);
+            };
+            if (!shares || my_steps == 0) release();
             const int first = S::OVERLAP && acc == 0 ? STEPS - 1 : 0;
 #pragma unroll 1
-            for (int i = 0; i < STEPS; ++i) {
-                const int c0 = (first + i) % STEPS * STEP;
+            for (int i = 0; i < my_steps; ++i) {
+                const int c0 = half * HALF + (first + i) % STEPS * STEP;
                 uint32_t r[STEP / 32][32];
 #pragma unroll
                 for (int h = 0; h < STEP / 32; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
                 tmem_ld_wait();
-                if (i == (S::OVERLAP ? 0 : STEPS - 1)) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_leader(&sh->tmem_empty[acc]);
-                }
+                if (shares && i == (S::OVERLAP ? 0 : STEPS - 1)) release();
 #pragma unroll
                 for (int h = 0; h < STEP / 32; ++h) {
                     const int c = c0 + 32 * h;
@@ -458,8 +461,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         alignas(16) OT o[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) o[j] = from_f32<OT>(v[j]);
-                        uint8_t *buf = sOut + ((warp - 2) * 2 + (stores & 1)) * OUT_BYTES;
-                        tma_store_wait_read<1>();  // the store before the last one has read its buffer
+                        uint8_t *buf = sOut + (warp - 2) * OUT_BYTES;
+                        tma_store_wait_read<0>();  // the last store has read the buffer
                         __syncwarp();
                         // 32 rows of 32 columns, 16-byte chunks swizzled as the tensor map says: 128-byte rows of fp32
                         // (chunk ^ row % 8), 64-byte rows of 16-bit outputs (chunk ^ row / 2 % 4)
@@ -477,7 +480,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 tma_store_3d(&tmOut, buf, un.col0 + c, row_w, un.split);
                             tma_store_commit();
                         }
-                        ++stores;
                     }
                 }
             }
@@ -489,28 +491,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!SWAP) tma_store_wait_read<0>();  // the buffers go with the CTA
     } else {
         // ---------------------------------------------------------------- scales (both CTAs)
+        // A group's words are loaded while the one before waits for its slot: a load from HBM takes as long
+        // as the MMAs of a group.
+        constexpr int WORDS = 1 + S::COL_WORDS / 4;
+        int u = first_unit, g = 0;
+        Unit un = unit_of<S>(p, u < units ? u : 0);
+        g = un.kb0 / 4;
+        uint4 w[WORDS];
+        auto load = [&]() {
+            w[0] = scale_words(p.r_scales, p.r_pitch, p.r_shift, un.row0 + (int)rank * kRowTile, p.rows, g, lane);
+#pragma unroll
+            for (int i = 1; i < WORDS; ++i)
+                w[i] = scale_words(p.c_scales, p.c_pitch, p.c_shift, un.col0 + 128 * (i - 1), p.cols, g, lane);
+        };
         int slot = 0;
         uint32_t phase = 0;
-        bool ok = true;
-        for (int u = first_unit; ok && u < units; u += step_units) {
-            const Unit un = unit_of<S>(p, u);
-            for (int g = un.kb0 / 4; 4 * g < un.kb1; ++g) {
-                uint4 w[1 + S::COL_WORDS / 4];
-                w[0] = scale_words(p.r_scales, p.r_pitch, p.r_shift, un.row0 + (int)rank * kRowTile, p.rows, g, lane);
+        if (u < units) load();
+        while (u < units) {
+            uint4 now[WORDS];
 #pragma unroll
-                for (int i = 0; i < S::COL_WORDS / 4; ++i)
-                    w[1 + i] = scale_words(p.c_scales, p.c_pitch, p.c_shift, un.col0 + 128 * i, p.cols, g, lane);
-                if (!(ok = wait(&sh->scale_empty[slot], phase ^ 1u))) break;
-                uint8_t *dst = sScale + slot * S::SLOT_BYTES + lane * 16;
-#pragma unroll
-                for (int i = 0; i < 1 + S::COL_WORDS / 4; ++i) *reinterpret_cast<uint4 *>(dst + 512 * i) = w[i];
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) arrive_leader(&sh->scale_full[slot]);
-                if (++slot == kScaleSlots) {
-                    slot = 0;
-                    phase ^= 1u;
+            for (int i = 0; i < WORDS; ++i) now[i] = w[i];
+            if (4 * ++g >= un.kb1) {
+                u += step_units;
+                if (u < units) {
+                    un = unit_of<S>(p, u);
+                    g = un.kb0 / 4;
                 }
+            }
+            if (u < units) load();
+            if (!wait(&sh->scale_empty[slot], phase ^ 1u)) break;
+            uint8_t *dst = sScale + slot * S::SLOT_BYTES + lane * 16;
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) *reinterpret_cast<uint4 *>(dst + 512 * i) = now[i];
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_leader(&sh->scale_full[slot]);
+            if (++slot == kScaleSlots) {
+                slot = 0;
+                phase ^= 1u;
             }
         }
     }
@@ -565,7 +583,7 @@ template <typename OT, typename S, bool SWAP>
 int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tmOut, const GemmParams &p,
            cudaStream_t stream) {
     auto kern = block_gemm_kernel<OT, S, SWAP>;
-    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + (SWAP ? 0 : 8 * 32 * 32 * sizeof(OT)) +
+    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + (SWAP ? 0 : kEpilogueWarps * 32 * 32 * sizeof(OT)) +
                             kScaleSlots * S::SLOT_BYTES + sizeof(Shared);
     static_assert(smem <= 232448, "shared memory per block");
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -749,8 +767,11 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     CUtensorMap tmR, tmC, tmOut = {};
     if ((st = make_map_e4m3(&tmR, R->data, (uint64_t)R->cols, (uint64_t)R->rows, (uint64_t)R->data_pitch, kRowTile)))
         return st;
-    if ((st = make_map_e4m3(&tmC, C->data, (uint64_t)C->cols, (uint64_t)C->rows, (uint64_t)C->data_pitch,
-                            pl.pair ? kPairCols / 2 : pl.cols)))
+    // A tile with fewer columns than its width loads only those (rows past a matrix cost TMA as much as rows
+    // of it); the rest of the stage holds anything, for sums that are never stored.
+    const int box = pl.pair ? kPairCols / 2 : std::min(pl.cols, cdiv(p.cols, 8) * 8);
+    p.col_bytes = box * kKBytes;
+    if ((st = make_map_e4m3(&tmC, C->data, (uint64_t)C->cols, (uint64_t)C->rows, (uint64_t)C->data_pitch, box)))
         return st;
     const int64_t es = (int64_t)dtype_size(dst.dtype);
     if (!pl.swap &&
