@@ -39,17 +39,6 @@ constexpr int kTmemCols = 512;
 constexpr int kPairCols = 256;                 // columns of a pair's tile
 constexpr int kRowTile = 128;                  // rows (TMEM lanes) per CTA
 
-// Division of n < 2^31 by a divisor d >= 1 known on the host: n / d = high 64 bits of n * (floor(2^64 / d) + 1)
-// (for d = 1 that does not fit 64 bits). A plain division is a chain of some 150 clocks,
-// and a tile's coordinates take four.
-struct Divisor {
-    unsigned long long magic;
-    int d;
-    __device__ __forceinline__ int div(int n) const {
-        return d == 1 ? n : (int)__umul64hi((unsigned long long)n, magic);
-    }
-};
-
 struct GemmParams {
     int rows, cols;            // of the tile grid: a's and b's, or b's and a's with SWAP
     int nkb, groups;           // K blocks of 128, and groups of four of them
@@ -106,15 +95,15 @@ struct Unit {
 template <typename S>
 __device__ __forceinline__ Unit unit_of(const GemmParams &p, int u) {
     Unit r;
-    r.split = p.by_tiles.div(u);
-    u -= r.split * p.by_tiles.d;
-    const int g = p.by_group.div(u);
+    r.split = (int)p.by_tiles.div(u);
+    u -= r.split * (int)p.by_tiles.d;
+    const int g = (int)p.by_group.div(u);
     const int first = g * p.group_rows;
     const bool last = p.row_tiles - first < p.group_rows;
     const Divisor by = last ? p.by_last_rows : p.by_rows;
-    const int local = u - g * p.by_group.d;
-    const int col = by.div(local);
-    r.row0 = (first + local - col * by.d) * S::ROWS;
+    const int local = u - g * (int)p.by_group.d;
+    const int col = (int)by.div(local);
+    r.row0 = (first + local - col * (int)by.d) * S::ROWS;
     r.col0 = col * S::COLS;
     r.kb0 = 4 * r.split * p.split_groups;
     r.kb1 = min(p.nkb, r.kb0 + 4 * p.split_groups);
@@ -652,8 +641,6 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool tma_out, int out_dtype) {
     return pl;
 }
 
-Divisor divisor(int d) { return Divisor{~0ull / (unsigned)d + 1, d}; }
-
 int64_t partial_pitch(int64_t N) { return (N + 3) / 4 * 4; }
 
 int check_product(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out) {
@@ -747,10 +734,10 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     // A group of row tiles runs side by side over each column tile: the columns' operand is read from HBM
     // once per group, while the group's 32 MB stay in L2.
     p.group_rows = (int)std::max<int64_t>(1, std::min<int64_t>(p.row_tiles, (int64_t(32) << 20) / (row_tile * a->cols)));
-    p.by_tiles = divisor(p.row_tiles * p.col_tiles);
-    p.by_group = divisor(p.group_rows * p.col_tiles);
-    p.by_rows = divisor(p.group_rows);
-    p.by_last_rows = divisor(p.row_tiles % p.group_rows ? p.row_tiles % p.group_rows : p.group_rows);
+    p.by_tiles = Divisor::of(p.row_tiles * p.col_tiles);
+    p.by_group = Divisor::of(p.group_rows * p.col_tiles);
+    p.by_rows = Divisor::of(p.group_rows);
+    p.by_last_rows = Divisor::of(p.row_tiles % p.group_rows ? p.row_tiles % p.group_rows : p.group_rows);
     p.r_scales = static_cast<const uint8_t *>(R->scales);
     p.c_scales = static_cast<const uint8_t *>(C->scales);
     p.r_pitch = R->scale_pitch;

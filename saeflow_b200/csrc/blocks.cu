@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sf_common.cuh"
 #include "sf_internal.h"
@@ -20,11 +21,6 @@ namespace {
 
 constexpr int kBlk = SF_BLOCK;
 
-// Magnitude bits of v where v is finite, else 0: ordered as integers like the magnitudes.
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;
-}
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
     const int s = (int)((amax_bits + 0x1FFFFFu) >> 23) - 8;
     return (uint32_t)max(s, 0);
@@ -33,21 +29,6 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
 __device__ __forceinline__ float inverse_scale(uint32_t s) { return __uint_as_float((254u - s) << 23); }
 __device__ __forceinline__ float scale_value(uint32_t s) { return __uint_as_float(s ? s << 23 : 0x00400000u); }
 
-// Four fp32 -> four e4m3 in one word. The conversion saturates, which in-range quotients never
-// meet; an infinity would become 448, so non-finite elements go in as NaN.
-__device__ __forceinline__ uint32_t pack_e4m3(const float *v, float inv) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float2 f;
-        f.x = v[2 * h] * inv;
-        f.y = v[2 * h + 1] * inv;
-        if ((__float_as_uint(v[2 * h]) & 0x7f800000u) == 0x7f800000u) f.x = __int_as_float(0x7fffffff);
-        if ((__float_as_uint(v[2 * h + 1]) & 0x7f800000u) == 0x7f800000u) f.y = __int_as_float(0x7fffffff);
-        w |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * h);
-    }
-    return w;
-}
 __device__ __forceinline__ void unpack_e4m3(uint32_t w, float *v) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -55,22 +36,6 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, float *v) {
         const float2 f = __half22float2(__half2(r));
         v[2 * h] = f.x;
         v[2 * h + 1] = f.y;
-    }
-}
-
-// Eight consecutive elements from column k of a row, zeros past K.
-template <typename XT>
-__device__ __forceinline__ void load8(const XT *row, int64_t k, int64_t K, int64_t sxk, bool vec, float (&v)[8]) {
-    if (vec && k + 8 <= K) {
-        uint4 q[sizeof(XT) / 2];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(XT) / 2; ++i) q[i] = __ldg(reinterpret_cast<const uint4 *>(row + k) + i);
-        const XT *e = reinterpret_cast<const XT *>(q);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_f32(__ldg(row + (k + j) * sxk)) : 0.f;
     }
 }
 
@@ -95,83 +60,253 @@ __device__ __forceinline__ void store8(uint8_t *row, int64_t k, int64_t limit, u
     }
 }
 
-// Row blocks: eight lanes to a block of 128, each with columns 8l..8l+7 and 64+8l..64+8l+7, so that
-// every load and store of the group is one contiguous run.
+// Sixteen of them, at a 16-byte aligned column.
+__device__ __forceinline__ void store16(uint8_t *row, int64_t k, int64_t limit, uint4 w) {
+    if (k + 16 <= limit) {
+        *reinterpret_cast<uint4 *>(row + k) = w;
+    } else {
+        store8(row, k, limit, make_uint2(w.x, w.y));
+        store8(row, k + 8, limit, make_uint2(w.z, w.w));
+    }
+}
+
+// Sixteen elements as a thread holds them: 16-bit types as eight words of two, fp32
+// as sixteen. Magnitudes compare as integers, two at a time in the 16-bit types.
+template <typename XT>
+struct Held {
+    static constexpr bool HALF = sizeof(XT) == 2;
+    static constexpr int WORDS = HALF ? 8 : 16;
+    static constexpr uint32_t ABS = HALF ? 0x7fff7fffu : 0x7fffffffu;
+    static __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return HALF ? __vmaxu2(a, b) : max(a, b); }
+    // fp32 value of element j of the words
+    static __device__ __forceinline__ float value(const uint32_t *w, int j) {
+        if constexpr (!HALF) {
+            return __uint_as_float(w[j]);
+        } else if constexpr (std::is_same_v<XT, __nv_bfloat16>) {
+            return __uint_as_float((j & 1) ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+        } else {
+            const __half2 h = *reinterpret_cast<const __half2 *>(&w[j >> 1]);
+            return (j & 1) ? __high2float(h) : __low2float(h);
+        }
+    }
+    // fp32 magnitude bits of half `j` of a word of magnitudes
+    static __device__ __forceinline__ uint32_t bits(uint32_t w, int j) { return __float_as_uint(value(&w, j)); }
+    static __device__ __forceinline__ uint32_t bits(uint32_t w) { return HALF ? max(bits(w, 0), bits(w, 1)) : w; }
+    // a word's magnitudes, 0 where they are not finite
+    static __device__ __forceinline__ uint32_t finite(uint32_t w) {
+        w &= ABS;
+        if constexpr (HALF) {
+            const uint32_t inf = std::is_same_v<XT, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+            return ((w & 0xffffu) < inf ? w & 0xffffu : 0u) | ((w >> 16) < inf ? w & 0xffff0000u : 0u);
+        } else {
+            return w < 0x7f800000u ? w : 0u;
+        }
+    }
+    // NaN in place of what is not finite
+    static __device__ __forceinline__ uint32_t nan_for_inf(uint32_t w) {
+        if constexpr (HALF) {
+            const uint32_t inf = std::is_same_v<XT, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+            return w | ((w & 0x7fffu) >= inf ? 0x7fffu : 0u) | (((w >> 16) & 0x7fffu) >= inf ? 0x7fff0000u : 0u);
+        } else {
+            return (w & 0x7fffffffu) >= 0x7f800000u ? 0x7fffffffu : w;
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Words of the 16 elements from column k of a row, zeros past K. `base` is the row's first element. Rows
+// with a unit column stride are read in aligned 16-byte pieces and shifted into place, so any alignment
+// of the element type costs one more piece and a few selects.
+template <typename XT>
+__device__ __forceinline__ void load16(const XT *base, int64_t k, int64_t K, int64_t sxk, uint32_t *v) {
+    using H = Held<XT>;
+    constexpr int W = H::WORDS, PER = 16 / W;
+    if (sxk == 1 && k + 16 <= K) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(base + k);
+        const uint4 *p = reinterpret_cast<const uint4 *>(at & ~uintptr_t(15));
+        const unsigned off = (unsigned)at & 15u;
+        if (off == 0) {
+#pragma unroll
+            for (int j = 0; j < W; j += 4) {
+                const uint4 a = __ldg(p + j / 4);
+                v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
+            }
+            return;
+        }
+        uint32_t w[W + 4];  // the last piece holds the last element, as off > 0
+#pragma unroll
+        for (int j = 0; j < W + 4; j += 4) {
+            const uint4 a = __ldg(p + j / 4);
+            w[j] = a.x, w[j + 1] = a.y, w[j + 2] = a.z, w[j + 3] = a.w;
+        }
+#pragma unroll
+        for (int j = 0; j < W + 2; ++j) w[j] = (off & 8) ? w[j + 2] : w[j];
+#pragma unroll
+        for (int j = 0; j < W + 1; ++j) w[j] = (off & 4) ? w[j + 1] : w[j];
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = H::HALF && (off & 2) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        XT e[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            e[i] = k + j * PER + i < K ? __ldg(base + (k + j * PER + i) * sxk) : from_f32<XT>(0.f);
+        if constexpr (PER == 1)
+            v[j] = __float_as_uint(to_f32(e[0]));
+        else
+            v[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(&e[0]) |
+                   (uint32_t)*reinterpret_cast<const uint16_t *>(&e[1]) << 16;
+    }
+}
+
+// Sixteen held elements times a scale, as e4m3.
+template <typename XT>
+__device__ __forceinline__ uint4 pack16(const uint32_t *v, float inv) {
+    using H = Held<XT>;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        w[j] = e4m3x2(H::value(v, 4 * j) * inv, H::value(v, 4 * j + 1) * inv) |
+               e4m3x2(H::value(v, 4 * j + 2) * inv, H::value(v, 4 * j + 3) * inv) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Row blocks: eight lanes to a block of 128, sixteen elements each; a group takes two blocks of a row
+// (`by` divides by the pairs of a row), so that enough bytes are on their way.
 template <typename XT>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const XT *__restrict__ x, int64_t n, int64_t K, int64_t sxm,
-                                                         int64_t sxk, bool vec, const int64_t *__restrict__ slots,
+                                                         int64_t sxk, const int64_t *__restrict__ slots,
                                                          uint8_t *__restrict__ q, int64_t q_pitch,
                                                          uint8_t *__restrict__ s, int64_t s_pitch, int64_t cap,
-                                                         unsigned nb, unsigned *err) {
+                                                         Divisor by, unsigned *err) {
+    using H = Held<XT>;
     const int l = threadIdx.x & 7;
-    const uint64_t item = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-    if (item >= (uint64_t)n * nb) return;  // whole groups leave together
+    const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
+    const int64_t row = by.div(item);
+    if (row >= n) return;  // whole groups leave together
     const unsigned group = 0xffu << (threadIdx.x & 24);
-    const int64_t row = (int64_t)(item / nb);
-    const unsigned blk = (unsigned)(item - (uint64_t)row * nb);
+    const int64_t pair = item - row * by.d;
     int64_t slot = row;
     if (slots) {
         slot = __ldg(slots + row);
-        if (slot >= cap && l == 0 && blk == 0) atomicOr(err, kErrIndex);
+        if (slot >= cap && l == 0 && pair == 0) atomicOr(err, kErrIndex);
         if (slot < 0 || slot >= cap) return;
     }
-    const int64_t k0 = (int64_t)blk * kBlk + 8 * l;
-    float a[8], b[8];
-    load8(x + row * sxm, k0, K, sxk, vec, a);
-    load8(x + row * sxm, k0 + 64, K, sxk, vec, b);
-    uint32_t m = 0;
+    uint32_t v[2][H::WORDS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, max(finite_bits(a[j]), finite_bits(b[j])));
+    for (int b = 0; b < 2; ++b) {
+        const int64_t k = (2 * pair + b) * kBlk + 16 * l;
+        load16(x + row * sxm, k, K, sxk, v[b]);
+    }
 #pragma unroll
-    for (int d = 4; d; d >>= 1) m = max(m, __shfl_xor_sync(group, m, d));
-    const uint32_t sb = scale_byte(m);
-    const float inv = inverse_scale(sb);
-    uint8_t *dst = q + slot * q_pitch;
-    store8(dst, k0, K, make_uint2(pack_e4m3(a, inv), pack_e4m3(a + 4, inv)));
-    store8(dst, k0 + 64, K, make_uint2(pack_e4m3(b, inv), pack_e4m3(b + 4, inv)));
-    if (l == 0) s[slot * s_pitch + blk] = (uint8_t)sb;
+    for (int b = 0; b < 2; ++b) {
+        const int64_t blk = 2 * pair + b;
+        if (blk * kBlk >= K) break;
+        uint32_t m = v[b][0] & H::ABS;
+#pragma unroll
+        for (int j = 1; j < H::WORDS; ++j) m = H::umax(m, v[b][j] & H::ABS);
+#pragma unroll
+        for (int d = 4; d; d >>= 1) m = H::umax(m, __shfl_xor_sync(group, m, d));
+        uint32_t bits = H::bits(m);
+        if (bits >= 0x7f800000u) {  // the group's: look at each element
+            m = 0;
+#pragma unroll
+            for (int j = 0; j < H::WORDS; ++j) {
+                m = H::umax(m, H::finite(v[b][j]));
+                v[b][j] = H::nan_for_inf(v[b][j]);
+            }
+#pragma unroll
+            for (int d = 4; d; d >>= 1) m = H::umax(m, __shfl_xor_sync(group, m, d));
+            bits = H::bits(m);
+        }
+        const uint32_t sb = scale_byte(bits);
+        store16(q + slot * q_pitch, blk * kBlk + 16 * l, K, pack16<XT>(v[b], inverse_scale(sb)));
+        if (l == 0) s[slot * s_pitch + blk] = (uint8_t)sb;
+    }
 }
 
-// Dequantising gather: the same lanes as above; `tile_shift` is 7 where a scale row serves 128 rows.
-template <typename OT>
+// Dequantising gather. A thread writes 16 aligned bytes of an output row, E elements, from the E numbers
+// there: `shift` elements of the row lie before its first 16-byte boundary, so piece c covers columns
+// c E - shift ... With shift = 0 a piece lies in one block; otherwise it may span two, with two scales.
+// PIECES pieces a thread, `stride` apart, so that enough bytes are on their way. `tile_shift` is 7 where a
+// scale row serves 128 rows.
+template <typename OT, bool ALIGNED>
 __global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t *__restrict__ q, int64_t q_pitch,
                                                         const uint8_t *__restrict__ s, int64_t s_pitch,
                                                         int64_t src_rows, int64_t K, int tile_shift,
                                                         const int64_t *__restrict__ rows, OT *__restrict__ out,
-                                                        int64_t n, int64_t out_pitch, bool vec, unsigned nb,
-                                                        unsigned *err) {
-    const int l = threadIdx.x & 7;
-    const uint64_t item = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-    if (item >= (uint64_t)n * nb) return;
-    const int64_t i = (int64_t)(item / nb);
-    const unsigned blk = (unsigned)(item - (uint64_t)i * nb);
+                                                        int64_t n, int64_t out_pitch, Divisor by, unsigned *err) {
+    constexpr int E = 16 / sizeof(OT), PIECES = 4;
+    const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t i = by.div(item);
+    if (i >= n) return;
+    const int64_t c = item - i * by.d;
     int64_t row = i;
     if (rows) {
         row = __ldg(rows + i);
-        if (row >= src_rows && l == 0 && blk == 0) atomicOr(err, kErrIndex);
+        if (row >= src_rows && c == 0) atomicOr(err, kErrIndex);
     }
     const bool have = row >= 0 && row < src_rows;
-    const float scale = have ? scale_value(__ldg(s + (row >> tile_shift) * s_pitch + blk)) : 0.f;
+    const uint8_t *src = q + row * q_pitch, *sc = s + (row >> tile_shift) * s_pitch;
     OT *dst = out + i * out_pitch;
+    const int shift = ALIGNED ? 0 : (int)((reinterpret_cast<uintptr_t>(dst) & 15u) / sizeof(OT));
+    uint2 w[PIECES];
+    uint32_t sb[PIECES][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int64_t k = (int64_t)blk * kBlk + 64 * h + 8 * l;
-        if (k >= K) break;
-        const uint2 w = have ? load8_e4m3(q + row * q_pitch, k, K) : make_uint2(0u, 0u);
-        float v[8];
-        unpack_e4m3(w.x, v);
-        unpack_e4m3(w.y, v + 4);
-        OT o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = from_f32<OT>(have ? v[j] * scale : 0.f);
-        if (vec && k + 8 <= K) {
-            const uint4 *src = reinterpret_cast<const uint4 *>(o);
-#pragma unroll
-            for (int j = 0; j < (int)sizeof(OT) / 2; ++j) reinterpret_cast<uint4 *>(dst + k)[j] = src[j];
+    for (int p = 0; p < PIECES; ++p) {
+        const int64_t k = (c + p * by.d) * E - shift;  // may start before the row, or end past it
+        w[p] = make_uint2(0u, 0u);
+        sb[p][0] = sb[p][1] = 0;
+        if (!have || k >= K || k + E <= 0) continue;
+        const int64_t last = min(k + E, K) - 1;
+        sb[p][0] = __ldg(sc + max(k, (int64_t)0) / kBlk);
+        if (!ALIGNED) sb[p][1] = __ldg(sc + last / kBlk);
+        if (ALIGNED && k + E <= K) {
+            if (E == 8)
+                w[p] = __ldg(reinterpret_cast<const uint2 *>(src + k));
+            else
+                w[p].x = __ldg(reinterpret_cast<const uint32_t *>(src + k));
+        } else if (!ALIGNED && (k & ~int64_t(3)) >= 0 && (k & ~int64_t(3)) + E + 4 <= K) {
+            const uint32_t *a = reinterpret_cast<const uint32_t *>(src + (k & ~int64_t(3)));
+            const uint32_t a0 = __ldg(a), a1 = __ldg(a + 1), a2 = E == 8 ? __ldg(a + 2) : 0u;
+            const int bits = 8 * (int)(k & 3);
+            w[p].x = __funnelshift_r(a0, a1, bits);
+            w[p].y = __funnelshift_r(a1, a2, bits);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k + j < K) dst[k + j] = o[j];
+            for (int j = 0; j < E; ++j)
+                if (k + j >= 0 && k + j < K) {
+                    const uint32_t byte = (uint32_t)__ldg(src + k + j) << (8 * (j & 3));
+                    if (j < 4)
+                        w[p].x |= byte;
+                    else
+                        w[p].y |= byte;
+                }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int64_t k = (c + p * by.d) * E - shift;
+        if (k >= K) break;
+        float v[8];
+        unpack_e4m3(w[p].x, v);
+        if (E == 8) unpack_e4m3(w[p].y, v + 4);
+        const float s0 = have ? scale_value(sb[p][0]) : 0.f, s1 = ALIGNED ? s0 : have ? scale_value(sb[p][1]) : 0.f;
+        const int64_t turn = (k + E - 1) / kBlk * kBlk;  // columns from here have the second scale
+        alignas(16) OT o[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] = from_f32<OT>(v[j] * (ALIGNED || k + j < turn ? s0 : s1));
+        if (k >= 0 && k + E <= K) {
+            *reinterpret_cast<uint4 *>(dst + k) = *reinterpret_cast<const uint4 *>(o);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (k + j >= 0 && k + j < K) dst[k + j] = o[j];
         }
     }
 }
@@ -197,109 +332,146 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint8_t *__restric
 }
 
 // One 128 x 128 tile of x per block, read once, for both orientations. Thread t of warp w holds rows
-// 16w + 4(lane / 8) + 0..3 and columns 8(lane % 8) + 0..7 (and + 64): four rows of a column make one
-// word of the transpose, which goes through shared memory (pitch 33 words) to be written by rows.
+// 16w + 4(lane / 8) + 0..3 and columns 16(lane % 8) + 0..15, in the input's type: a row's 16 results are
+// one 16-byte store, and four rows of a column make one word of the transpose, which goes through shared
+// memory (16-byte chunks swizzled by the column) to be written by rows. The elements are looked at in
+// pairs for the maxima; only a tile that holds an infinity or NaN looks at each of them.
 template <typename XT, bool TILE>
-__global__ void __launch_bounds__(256) quant_tile_kernel(const XT *__restrict__ x, int64_t R, int64_t C, int64_t sxm,
-                                                         int64_t sxk, bool vec, uint8_t *__restrict__ q,
-                                                         int64_t q_pitch, uint8_t *__restrict__ qs, int64_t qs_pitch,
-                                                         uint8_t *__restrict__ t, int64_t t_pitch,
-                                                         uint8_t *__restrict__ ts, int64_t ts_pitch,
-                                                         float *__restrict__ sums) {
-    __shared__ uint32_t trans[kBlk * 33];
-    __shared__ uint32_t col_max[kBlk];
+__global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
+    quant_tile_kernel(const XT *__restrict__ x, int64_t R, int64_t C, int64_t sxm, int64_t sxk, uint8_t *__restrict__ q,
+                      int64_t q_pitch, uint8_t *__restrict__ qs, int64_t qs_pitch,
+                      uint8_t *__restrict__ t, int64_t t_pitch, uint8_t *__restrict__ ts, int64_t ts_pitch,
+                      float *__restrict__ sums) {
+    using H = Held<XT>;
+    constexpr int W = H::WORDS, PER = 16 / W;  // words of 16 elements, elements of a word
+    __shared__ __align__(16) uint32_t trans[kBlk * 32];
+    __shared__ __align__(16) float col_inv[kBlk];
+    __shared__ uint32_t col_max[8][kBlk / PER];
     __shared__ float col_sum[8][kBlk];
-    __shared__ uint32_t tile_max;
+    __shared__ uint32_t warp_max[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 7;
     const int64_t rb = blockIdx.y, cb = blockIdx.x;
     const int rl = 16 * warp + 4 * (lane >> 3);
-    const int64_t r0 = rb * kBlk + rl, c0 = cb * kBlk + 8 * l;
-    if (threadIdx.x < kBlk) col_max[threadIdx.x] = 0;
-    if (threadIdx.x == 0) tile_max = 0;
-    __syncthreads();
-    float v[4][16];
+    const int64_t r0 = rb * kBlk + rl, c0 = cb * kBlk + 16 * l;
+
+    uint32_t v[4][W];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float(&lo)[8] = *reinterpret_cast<float(*)[8]>(&v[i][0]);
-        float(&hi)[8] = *reinterpret_cast<float(*)[8]>(&v[i][8]);
-        if (r0 + i < R) {
-            load8(x + (r0 + i) * sxm, c0, C, sxk, vec, lo);
-            load8(x + (r0 + i) * sxm, c0 + 64, C, sxk, vec, hi);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[i][j] = 0.f;
-        }
-    }
-    uint32_t rm[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        rm[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) rm[i] = max(rm[i], finite_bits(v[i][j]));
-#pragma unroll
-        for (int d = 4; d; d >>= 1) rm[i] = max(rm[i], __shfl_xor_sync(0xffffffffu, rm[i], d));
-    }
-    if (TILE) {
-        if (l == 0) atomicMax(&tile_max, max(max(rm[0], rm[1]), max(rm[2], rm[3])));
-    } else if (t) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            uint32_t m = max(max(finite_bits(v[0][j]), finite_bits(v[1][j])),
-                             max(finite_bits(v[2][j]), finite_bits(v[3][j])));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            if (lane < 8) atomicMax(&col_max[8 * l + (j & 7) + 64 * (j >> 3)], m);
-        }
-    }
+    for (int i = 0; i < 4; ++i) load16(x + (r0 + i) * sxm, c0, r0 + i < R ? C : 0, sxk, v[i]);
     if (sums) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            float a = (v[0][j] + v[1][j]) + (v[2][j] + v[3][j]);
+            float a = (H::value(v[0], j) + H::value(v[1], j)) + (H::value(v[2], j) + H::value(v[3], j));
             a += __shfl_xor_sync(0xffffffffu, a, 8);
             a += __shfl_xor_sync(0xffffffffu, a, 16);
-            if (lane < 8) col_sum[warp][8 * l + (j & 7) + 64 * (j >> 3)] = a;
+            if (lane < 8) col_sum[warp][16 * l + j] = a;
+        }
+    }
+    uint32_t rm[4];  // fp32 magnitude bits of each row's maximum
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t m = v[i][0] & H::ABS;
+#pragma unroll
+        for (int j = 1; j < W; ++j) m = H::umax(m, v[i][j] & H::ABS);
+#pragma unroll
+        for (int d = 4; d; d >>= 1) m = H::umax(m, __shfl_xor_sync(0xffffffffu, m, d));
+        rm[i] = H::bits(m);
+        odd |= rm[i] >= 0x7f800000u;
+    }
+    const bool not_finite = __syncthreads_or(odd);
+    uint32_t cm[W];  // magnitudes of each column's maximum over this thread's rows
+    if (not_finite) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < W; ++j) m = H::umax(m, H::finite(v[i][j]));
+#pragma unroll
+            for (int d = 4; d; d >>= 1) m = H::umax(m, __shfl_xor_sync(0xffffffffu, m, d));
+            rm[i] = H::bits(m);
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            cm[j] = H::umax(H::umax(H::finite(v[0][j]), H::finite(v[1][j])),
+                            H::umax(H::finite(v[2][j]), H::finite(v[3][j])));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i][j] = H::nan_for_inf(v[i][j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            cm[j] = H::umax(H::umax(v[0][j] & H::ABS, v[1][j] & H::ABS), H::umax(v[2][j] & H::ABS, v[3][j] & H::ABS));
+    }
+    if (TILE) {
+        uint32_t m = max(max(rm[0], rm[1]), max(rm[2], rm[3]));
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0) warp_max[warp] = m;
+    } else if (t) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            uint32_t m = H::umax(cm[j], __shfl_xor_sync(0xffffffffu, cm[j], 8));
+            m = H::umax(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            if (lane < 8) col_max[warp][W * l + j] = m;
         }
     }
     __syncthreads();
+    uint32_t tile_byte = 0;
+    if (TILE) {
+        uint32_t m = warp_max[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) m = max(m, warp_max[w]);
+        tile_byte = scale_byte(m);
+    }
+    if (threadIdx.x < kBlk) {
+        const int c = threadIdx.x;
+        const int64_t col = cb * kBlk + c;
+        if (!TILE && t) {
+            uint32_t m = col_max[0][c / PER];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) m = H::umax(m, col_max[w][c / PER]);
+            const uint32_t sb = scale_byte(H::bits(m, PER == 1 ? 0 : c & 1));
+            col_inv[c] = inverse_scale(sb);
+            if (col < C) ts[col * ts_pitch + rb] = (uint8_t)sb;
+        }
+        if (sums && col < C) {
+            float a = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) a += col_sum[w][c];
+            sums[rb * C + col] = a;
+        }
+    }
+    if (TILE && threadIdx.x == 0) {
+        if (q) qs[rb * qs_pitch + cb] = (uint8_t)tile_byte;
+        if (t) ts[cb * ts_pitch + rb] = (uint8_t)tile_byte;
+    }
     if (q) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (r0 + i >= R) break;
-            const uint32_t sb = scale_byte(TILE ? tile_max : rm[i]);
-            const float inv = inverse_scale(sb);
-            uint8_t *dst = q + (r0 + i) * q_pitch;
-            store8(dst, c0, C, make_uint2(pack_e4m3(&v[i][0], inv), pack_e4m3(&v[i][4], inv)));
-            store8(dst, c0 + 64, C, make_uint2(pack_e4m3(&v[i][8], inv), pack_e4m3(&v[i][12], inv)));
+            const uint32_t sb = TILE ? tile_byte : scale_byte(rm[i]);
+            store16(q + (r0 + i) * q_pitch, c0, C, pack16<XT>(v[i], inverse_scale(sb)));
             if (!TILE && l == 0) qs[(r0 + i) * qs_pitch + cb] = (uint8_t)sb;
         }
-        if (TILE && threadIdx.x == 0) qs[rb * qs_pitch + cb] = (uint8_t)scale_byte(tile_max);
-    }
-    if (sums && threadIdx.x < kBlk && cb * kBlk + threadIdx.x < C) {
-        float a = 0.f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) a += col_sum[w][threadIdx.x];
-        sums[rb * C + cb * kBlk + threadIdx.x] = a;
     }
     if (!t) return;
+    if (!TILE) __syncthreads();  // col_inv
+    const float tile_inv = inverse_scale(tile_byte);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-        const int c = 8 * l + (j & 7) + 64 * (j >> 3);
-        const float inv = inverse_scale(scale_byte(TILE ? tile_max : col_max[c]));
-        const float col[4] = {v[0][j], v[1][j], v[2][j], v[3][j]};
-        trans[c * 33 + (rl >> 2)] = pack_e4m3(col, inv);
+        const int c = 16 * l + j;
+        const float inv = TILE ? tile_inv : col_inv[c];
+        trans[c * 32 + ((warp ^ l) << 2 | (lane >> 3))] =
+            e4m3x2(H::value(v[0], j) * inv, H::value(v[1], j) * inv) |
+            e4m3x2(H::value(v[2], j) * inv, H::value(v[3], j) * inv) << 16;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int c = 32 * i + 4 * warp + (lane >> 3);
         if (cb * kBlk + c >= C) break;
-        const uint32_t *src = &trans[c * 33 + 4 * l];
-        uint8_t *dst = t + (cb * kBlk + c) * t_pitch;
-        store8(dst, rb * kBlk + 16 * l, R, make_uint2(src[0], src[1]));
-        store8(dst, rb * kBlk + 16 * l + 8, R, make_uint2(src[2], src[3]));
-        if (!TILE && l == 0) ts[(cb * kBlk + c) * ts_pitch + rb] = (uint8_t)scale_byte(col_max[c]);
+        const uint4 w = *reinterpret_cast<const uint4 *>(&trans[c * 32 + ((l ^ (c >> 4)) << 2)]);
+        store16(t + (cb * kBlk + c) * t_pitch, rb * kBlk + 16 * l, R, w);
     }
-    if (TILE && threadIdx.x == 0) ts[cb * ts_pitch + rb] = (uint8_t)scale_byte(tile_max);
 }
 
 // col_sums[c] = the partial sums of the row blocks, in order.
@@ -377,16 +549,16 @@ int sf_blocks_write(const sf_matrix *x, const int64_t *slots, const sf_blocks *d
                          (long long)dst->cols);
     if (!slots && x->rows > dst->rows) return set_error(SF_ERR_INVALID, "x has more rows than dst");
     if (x->rows == 0 || x->cols == 0) return SF_OK;
-    const unsigned nb = (unsigned)((x->cols + kBlk - 1) / kBlk);
+    const Divisor by = Divisor::of((x->cols + 2 * kBlk - 1) / (2 * kBlk));
     unsigned grid = 0;
-    if ((st = grid_for((uint64_t)x->rows * nb, 8, &grid))) return st;
+    if ((st = grid_for((uint64_t)x->rows * by.d, 8, &grid))) return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return with_type(x->dtype, [&](auto tag) {
         using T = decltype(tag);
         quant_rows_kernel<T><<<grid, 256, 0, s>>>(
-            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col, vector_rows(*x),
-            slots, static_cast<uint8_t *>(dst->data), dst->data_pitch, static_cast<uint8_t *>(dst->scales),
-            dst->scale_pitch, dst->rows, nb, device_error_word());
+            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col, slots,
+            static_cast<uint8_t *>(dst->data), dst->data_pitch, static_cast<uint8_t *>(dst->scales), dst->scale_pitch,
+            dst->rows, by, device_error_word());
         return check_cuda(cudaGetLastError(), "quant_rows launch");
     });
 }
@@ -399,17 +571,20 @@ int sf_blocks_read(const sf_blocks *src, const int64_t *rows, const sf_matrix *o
     if (!rows && out->rows > src->rows) return set_error(SF_ERR_INVALID, "out has more rows than src");
     if (out->rows == 0 || out->cols == 0) return SF_OK;
     if (out->stride_col != 1) return set_error(SF_ERR_UNSUPPORTED, "out needs a unit column stride");
-    const unsigned nb = (unsigned)((src->cols + kBlk - 1) / kBlk);
+    const bool aligned = vector_rows(*out);
+    // a row's pieces of 16 bytes (one more where rows start between boundaries), four to a thread
+    const int64_t pieces = (out->cols * (int64_t)dtype_size(out->dtype) + 15) / 16 + (aligned ? 0 : 1);
+    const Divisor by = Divisor::of((pieces + 3) / 4);
     unsigned grid = 0;
-    if ((st = grid_for((uint64_t)out->rows * nb, 8, &grid))) return st;
+    if ((st = grid_for((uint64_t)out->rows * by.d, 1, &grid))) return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return with_type(out->dtype, [&](auto tag) {
         using T = decltype(tag);
-        read_rows_kernel<T><<<grid, 256, 0, s>>>(
+        auto kern = aligned ? read_rows_kernel<T, true> : read_rows_kernel<T, false>;
+        kern<<<grid, 256, 0, s>>>(
             static_cast<const uint8_t *>(src->data), src->data_pitch, static_cast<const uint8_t *>(src->scales),
             src->scale_pitch, src->rows, src->cols, src->tile ? 7 : 0, rows,
-            reinterpret_cast<T *>(const_cast<void *>(out->data)), out->rows, out->stride_row, vector_rows(*out), nb,
-            device_error_word());
+            reinterpret_cast<T *>(const_cast<void *>(out->data)), out->rows, out->stride_row, by, device_error_word());
         return check_cuda(cudaGetLastError(), "read_rows launch");
     });
 }
@@ -472,7 +647,7 @@ int sf_blocks_quantize(const sf_matrix *x, const sf_blocks *q, const sf_blocks *
         using T = decltype(tag);
         auto kern = tile ? quant_tile_kernel<T, true> : quant_tile_kernel<T, false>;
         kern<<<dim3((unsigned)ncb, (unsigned)nrb), 256, 0, s>>>(
-            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col, vector_rows(*x),
+            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col,
             static_cast<uint8_t *>(a.data), a.data_pitch, static_cast<uint8_t *>(a.scales), a.scale_pitch,
             static_cast<uint8_t *>(b.data), b.data_pitch, static_cast<uint8_t *>(b.scales), b.scale_pitch, part);
         return check_cuda(cudaGetLastError(), "quant_tile launch");

@@ -61,6 +61,19 @@ __device__ __forceinline__ float round_to(float v, int dtype) {
 }
 
 // ---------------------------------------------------------------------------------------
+// Division of 0 <= n < 2^40 by a divisor 1 <= d < 2^24 known on the host: n / d is the high 64 bits of
+// n * (floor(2^64 / d) + 1), whose excess over 2^64 n / d is below n (the multiplier of d = 1 does not
+// fit 64 bits). A plain 64-bit division takes about a hundred instructions.
+struct Divisor {
+    unsigned long long magic;
+    int64_t d;
+    __host__ static Divisor of(int64_t d) { return Divisor{~0ull / (unsigned long long)d + 1, d}; }
+    __device__ __forceinline__ int64_t div(int64_t n) const {
+        return d == 1 ? n : (int64_t)__umul64hi((unsigned long long)n, magic);
+    }
+};
+
+// ---------------------------------------------------------------------------------------
 // Shared-memory addressing, timers
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
