@@ -197,11 +197,23 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const XT *__restrict__ 
         if (slot >= cap && l == 0 && pair == 0) atomicOr(err, kErrIndex);
         if (slot < 0 || slot >= cap) return;
     }
+    // Sixteen columns from 16l; of aligned fp32 rows four from 4l of each 32, so that the group's 16-byte loads
+    // are side by side.
+    const XT *src = x + row * sxm;
+    const bool quads = !H::HALF && sxk == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0 && (2 * pair + 2) * kBlk <= K;
     uint32_t v[2][H::WORDS];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const int64_t k = (2 * pair + b) * kBlk + 16 * l;
-        load16(x + row * sxm, k, K, sxk, v[b]);
+        const int64_t k = (2 * pair + b) * kBlk;
+        if (!H::HALF && quads) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint4 a = __ldg(reinterpret_cast<const uint4 *>(src + k) + 8 * j + l);
+                v[b][4 * j] = a.x, v[b][4 * j + 1] = a.y, v[b][4 * j + 2] = a.z, v[b][4 * j + 3] = a.w;
+            }
+        } else {
+            load16(src, k + 16 * l, K, sxk, v[b]);
+        }
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -225,27 +237,40 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const XT *__restrict__ 
             bits = H::bits(m);
         }
         const uint32_t sb = scale_byte(bits);
-        store16(q + slot * q_pitch, blk * kBlk + 16 * l, K, pack16<XT>(v[b], inverse_scale(sb)));
+        uint8_t *dst = q + slot * q_pitch;
+        const uint4 w = pack16<XT>(v[b], inverse_scale(sb));
+        if (!H::HALF && quads) {
+            uint32_t *to = reinterpret_cast<uint32_t *>(dst + blk * kBlk) + l;
+            to[0] = w.x, to[8] = w.y, to[16] = w.z, to[24] = w.w;
+        } else {
+            store16(dst, blk * kBlk + 16 * l, K, w);
+        }
         if (l == 0) s[slot * s_pitch + blk] = (uint8_t)sb;
     }
 }
 
-// Dequantising gather. A thread writes 16 aligned bytes of an output row, E elements, from the E numbers
-// there: `shift` elements of the row lie before its first 16-byte boundary, so piece c covers columns
-// c E - shift ... With shift = 0 a piece lies in one block; otherwise it may span two, with two scales.
-// PIECES pieces a thread, `stride` apart, so that enough bytes are on their way. `tile_shift` is 7 where a
-// scale row serves 128 rows.
+// Output elements of a thread of read_rows_kernel, eight to a piece. 16-bit outputs, 16384 rows of 2304 from a
+// store of 262144: 22.5 us with 16, 19.9 with 32, 21.9 with 64; fp32, 65536 rows: 147, 141 and 145 us with 8,
+// 16 and 32.
+template <typename OT>
+constexpr int kReadElements = sizeof(OT) == 4 ? 16 : 32;
+
+// Dequantising gather. A piece is eight numbers on their way to an aligned place of an output row (16 bytes of a
+// 16-bit type, 32 of fp32 by two stores): `shift` elements of the row lie before its first 16-byte boundary,
+// so piece c covers columns 8c - shift ... With shift = 0 a piece lies in one block; otherwise it may span
+// two, with two scales. Eight lanes take eight neighbouring pieces at a time and several times over, so
+// that enough bytes are on their way. `tile_shift` is 7 where a scale row serves 128 rows.
 template <typename OT, bool ALIGNED>
 __global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t *__restrict__ q, int64_t q_pitch,
                                                         const uint8_t *__restrict__ s, int64_t s_pitch,
                                                         int64_t src_rows, int64_t K, int tile_shift,
                                                         const int64_t *__restrict__ rows, OT *__restrict__ out,
                                                         int64_t n, int64_t out_pitch, Divisor by, unsigned *err) {
-    constexpr int E = 16 / sizeof(OT), PIECES = 4;
-    const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t i = by.div(item);
+    constexpr int PIECES = kReadElements<OT> / 8;
+    const int64_t group = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
+    const int64_t i = by.div(group);
     if (i >= n) return;
-    const int64_t c = item - i * by.d;
+    const int64_t c = (group - i * by.d) * 8 * PIECES + (threadIdx.x & 7);
     int64_t row = i;
     if (rows) {
         row = __ldg(rows + i);
@@ -259,27 +284,22 @@ __global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t *__restric
     uint32_t sb[PIECES][2];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int64_t k = (c + p * by.d) * E - shift;  // may start before the row, or end past it
+        const int64_t k = (c + 8 * p) * 8 - shift;  // may start before the row, or end past it
         w[p] = make_uint2(0u, 0u);
         sb[p][0] = sb[p][1] = 0;
-        if (!have || k >= K || k + E <= 0) continue;
-        const int64_t last = min(k + E, K) - 1;
+        if (!have || k >= K || k + 8 <= 0) continue;
         sb[p][0] = __ldg(sc + max(k, (int64_t)0) / kBlk);
-        if (!ALIGNED) sb[p][1] = __ldg(sc + last / kBlk);
-        if (ALIGNED && k + E <= K) {
-            if (E == 8)
-                w[p] = __ldg(reinterpret_cast<const uint2 *>(src + k));
-            else
-                w[p].x = __ldg(reinterpret_cast<const uint32_t *>(src + k));
-        } else if (!ALIGNED && (k & ~int64_t(3)) >= 0 && (k & ~int64_t(3)) + E + 4 <= K) {
+        if (!ALIGNED) sb[p][1] = __ldg(sc + (min(k + 8, K) - 1) / kBlk);
+        if (ALIGNED && k + 8 <= K) {
+            w[p] = __ldg(reinterpret_cast<const uint2 *>(src + k));
+        } else if (!ALIGNED && (k & ~int64_t(3)) >= 0 && (k & ~int64_t(3)) + 12 <= K) {
             const uint32_t *a = reinterpret_cast<const uint32_t *>(src + (k & ~int64_t(3)));
-            const uint32_t a0 = __ldg(a), a1 = __ldg(a + 1), a2 = E == 8 ? __ldg(a + 2) : 0u;
+            const uint32_t a0 = __ldg(a), a1 = __ldg(a + 1), a2 = __ldg(a + 2);
             const int bits = 8 * (int)(k & 3);
-            w[p].x = __funnelshift_r(a0, a1, bits);
-            w[p].y = __funnelshift_r(a1, a2, bits);
+            w[p] = make_uint2(__funnelshift_r(a0, a1, bits), __funnelshift_r(a1, a2, bits));
         } else {
 #pragma unroll
-            for (int j = 0; j < E; ++j)
+            for (int j = 0; j < 8; ++j)
                 if (k + j >= 0 && k + j < K) {
                     const uint32_t byte = (uint32_t)__ldg(src + k + j) << (8 * (j & 3));
                     if (j < 4)
@@ -291,21 +311,23 @@ __global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t *__restric
     }
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int64_t k = (c + p * by.d) * E - shift;
+        const int64_t k = (c + 8 * p) * 8 - shift;
         if (k >= K) break;
         float v[8];
         unpack_e4m3(w[p].x, v);
-        if (E == 8) unpack_e4m3(w[p].y, v + 4);
+        unpack_e4m3(w[p].y, v + 4);
         const float s0 = have ? scale_value(sb[p][0]) : 0.f, s1 = ALIGNED ? s0 : have ? scale_value(sb[p][1]) : 0.f;
-        const int64_t turn = (k + E - 1) / kBlk * kBlk;  // columns from here have the second scale
-        alignas(16) OT o[E];
+        const int64_t turn = (k + 7) / kBlk * kBlk;  // columns from here have the second scale
+        alignas(16) OT o[8];
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] = from_f32<OT>(v[j] * (ALIGNED || k + j < turn ? s0 : s1));
-        if (k >= 0 && k + E <= K) {
-            *reinterpret_cast<uint4 *>(dst + k) = *reinterpret_cast<const uint4 *>(o);
+        for (int j = 0; j < 8; ++j) o[j] = from_f32<OT>(v[j] * (ALIGNED || k + j < turn ? s0 : s1));
+        if (k >= 0 && k + 8 <= K) {
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(OT) / 2; ++j)  // streaming: 21.1 -> 19.9 us at the sizes above
+                __stcs(reinterpret_cast<uint4 *>(dst + k) + j, reinterpret_cast<const uint4 *>(o)[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < E; ++j)
+            for (int j = 0; j < 8; ++j)
                 if (k + j >= 0 && k + j < K) dst[k + j] = o[j];
         }
     }
@@ -344,10 +366,10 @@ __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
                       float *__restrict__ sums) {
     using H = Held<XT>;
     constexpr int W = H::WORDS, PER = 16 / W;  // words of 16 elements, elements of a word
-    __shared__ __align__(16) uint32_t trans[kBlk * 32];
+    __shared__ __align__(16) uint32_t trans[kBlk * 32];  // first the column sums of 32 groups of four rows
+    float *scratch = reinterpret_cast<float *>(trans);
     __shared__ __align__(16) float col_inv[kBlk];
     __shared__ uint32_t col_max[8][kBlk / PER];
-    __shared__ float col_sum[8][kBlk];
     __shared__ uint32_t warp_max[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 7;
     const int64_t rb = blockIdx.y, cb = blockIdx.x;
@@ -357,13 +379,15 @@ __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
     uint32_t v[4][W];
 #pragma unroll
     for (int i = 0; i < 4; ++i) load16(x + (r0 + i) * sxm, c0, r0 + i < R ? C : 0, sxk, v[i]);
-    if (sums) {
+    if (sums) {  // each thread's four rows; quad j of lane l at quad 4l + (j + l / 2) % 4, without bank conflicts
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            float a = (H::value(v[0], j) + H::value(v[1], j)) + (H::value(v[2], j) + H::value(v[3], j));
-            a += __shfl_xor_sync(0xffffffffu, a, 8);
-            a += __shfl_xor_sync(0xffffffffu, a, 16);
-            if (lane < 8) col_sum[warp][16 * l + j] = a;
+        for (int j = 0; j < 16; j += 4) {
+            float a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                a[e] = (H::value(v[0], j + e) + H::value(v[1], j + e)) + (H::value(v[2], j + e) + H::value(v[3], j + e));
+            *reinterpret_cast<float4 *>(&scratch[(rl >> 2) * kBlk + 16 * l + 4 * (((j >> 2) + (l >> 1)) & 3)]) =
+                make_float4(a[0], a[1], a[2], a[3]);
         }
     }
     uint32_t rm[4];  // fp32 magnitude bits of each row's maximum
@@ -434,9 +458,10 @@ __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
             if (col < C) ts[col * ts_pitch + rb] = (uint8_t)sb;
         }
         if (sums && col < C) {
+            const int at = (c & ~15) + 4 * (((c >> 2) + (c >> 5)) & 3) + (c & 3);
             float a = 0.f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) a += col_sum[w][c];
+            for (int g = 0; g < 32; ++g) a += scratch[g * kBlk + at];
             sums[rb * C + col] = a;
         }
     }
@@ -454,7 +479,7 @@ __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
         }
     }
     if (!t) return;
-    if (!TILE) __syncthreads();  // col_inv
+    if (!TILE || sums) __syncthreads();  // col_inv is written, scratch has been read
     const float tile_inv = inverse_scale(tile_byte);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -474,15 +499,26 @@ __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
     }
 }
 
-// col_sums[c] = the partial sums of the row blocks, in order.
+// col_sums[c] = the partial sums of the row blocks: 32 columns a block, eight ranges of row blocks summed in
+// order, then the ranges in order.
 __global__ void __launch_bounds__(256) join_sums_kernel(const float *__restrict__ part, int64_t nrb, int64_t C,
                                                         float *__restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= C) return;
+    __shared__ float range[8][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane, each = (nrb + 7) / 8;
     float a = 0.f;
+    if (c < C) {
 #pragma unroll 8
-    for (int64_t r = 0; r < nrb; ++r) a += __ldg(part + r * C + c);
-    out[c] = a;
+        for (int64_t r = w * each; r < min(nrb, (w + 1) * each); ++r) a += __ldg(part + r * C + c);
+    }
+    range[w][lane] = a;
+    __syncthreads();
+    if (w == 0 && c < C) {
+        a = range[0][lane];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) a += range[i][lane];
+        out[c] = a;
+    }
 }
 
 bool aligned_to(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
@@ -572,11 +608,12 @@ int sf_blocks_read(const sf_blocks *src, const int64_t *rows, const sf_matrix *o
     if (out->rows == 0 || out->cols == 0) return SF_OK;
     if (out->stride_col != 1) return set_error(SF_ERR_UNSUPPORTED, "out needs a unit column stride");
     const bool aligned = vector_rows(*out);
-    // a row's pieces of 16 bytes (one more where rows start between boundaries), four to a thread
-    const int64_t pieces = (out->cols * (int64_t)dtype_size(out->dtype) + 15) / 16 + (aligned ? 0 : 1);
-    const Divisor by = Divisor::of((pieces + 3) / 4);
+    // a row's pieces of eight, one more where rows start between boundaries
+    const int64_t pieces = (out->cols + 7) / 8 + (aligned ? 0 : 1);
+    const int64_t each = out->dtype == SF_F32 ? kReadElements<float> : kReadElements<__half>;  // 8 lanes, 8 a piece
+    const Divisor by = Divisor::of((pieces + each - 1) / each);
     unsigned grid = 0;
-    if ((st = grid_for((uint64_t)out->rows * by.d, 1, &grid))) return st;
+    if ((st = grid_for((uint64_t)out->rows * by.d, 8, &grid))) return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return with_type(out->dtype, [&](auto tag) {
         using T = decltype(tag);
@@ -653,7 +690,7 @@ int sf_blocks_quantize(const sf_matrix *x, const sf_blocks *q, const sf_blocks *
         return check_cuda(cudaGetLastError(), "quant_tile launch");
     });
     if (st || !col_sums) return st;
-    join_sums_kernel<<<(unsigned)((x->cols + 255) / 256), 256, 0, s>>>(part, nrb, x->cols, col_sums);
+    join_sums_kernel<<<(unsigned)((x->cols + 31) / 32), 256, 0, s>>>(part, nrb, x->cols, col_sums);
     return check_cuda(cudaGetLastError(), "join_sums launch");
 }
 

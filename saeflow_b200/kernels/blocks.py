@@ -28,6 +28,14 @@ def _cdiv(a, b):
     return -(-a // b)
 
 
+def _layout(rows, cols, tile):
+    """(data pitch, scale pitch, rows of scales, bytes of both from a 256-byte aligned start) of the smallest
+    aligned rows."""
+    dp, sp = _cdiv(cols, 16) * 16, _cdiv(cols, 4 * BLOCK) * 4
+    scale_rows = _cdiv(rows, BLOCK) if tile else rows
+    return dp, sp, scale_rows, _cdiv(rows * dp, 256) * 256 + _cdiv(scale_rows * sp, 256) * 256
+
+
 class BlockScaled:
     """An 8-bit matrix [rows, cols] on a CUDA device.
 
@@ -70,12 +78,17 @@ class BlockScaled:
         dev = torch.device("cuda" if device is None else device)
         if dev.type != "cuda":
             raise ValueError(f"device is {dev}; saeflow_b200 runs on CUDA devices only")
+        dp, sp, scale_rows, _ = _layout(rows, cols, tile)
+        data = torch.empty_strided((rows, cols), (dp, 1), dtype=_F8, device=dev)
+        # a product reads scale bytes four at a time, so the padding is there; its values are never used
+        scales = torch.empty(scale_rows, sp, dtype=torch.uint8, device=dev)
         nb = _cdiv(cols, BLOCK)
-        data = torch.empty(rows, _cdiv(cols, 16) * 16, dtype=_F8, device=dev)[:, :cols]
-        # a product reads scale bytes four at a time; the padding's values are never used
-        scales = torch.empty(_cdiv(rows, BLOCK) if tile else rows, _cdiv(nb, 4) * 4, dtype=torch.uint8,
-                             device=dev)[:, :nb]
-        return cls(data, scales, tile)
+        self = cls.__new__(cls)
+        self.data, self.scales = data, scales if sp == nb else scales[:, :nb]
+        self.tile, self.shape, self.device = bool(tile), (rows, cols), data.device
+        self._c = _abi.SfBlocks(data.data_ptr(), scales.data_ptr(), rows, cols, dp, sp, int(tile), 0)
+        self._ref = ctypes.byref(self._c)
+        return self
 
     def rows(self, start, stop):
         """Rows [start, stop) in place (row blocks only)."""
@@ -93,22 +106,27 @@ class BlockScaled:
 
 def _run(dev, fn, *args):
     """Call a library function on `dev`'s current stream."""
-    if torch.cuda.current_device() == dev.index:
-        _abi.check(fn(*args, _abi.stream_of(dev)))
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:  # as torch.cuda.current_device, on an initialised device
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
-            _abi.check(fn(*args, _abi.stream_of(dev)))
+            status = fn(*args, _abi.stream_of(dev))
+    if status:
+        _abi.check(status)
 
 
 def _index(t, name, n, dev):
     """`t` as a contiguous int64 tensor [n] on dev."""
     if t.dim() != 1 or n is not None and t.shape[0] != n:
         raise ValueError(f"{name} must be 1-D{'' if n is None else f' with {n} entries'}, got {tuple(t.shape)}")
-    if t.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"{name} has dtype {t.dtype}; expected int64 or int32")
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    return t.to(torch.int64).contiguous()
+    if t.dtype != torch.int64:
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} has dtype {t.dtype}; expected int64 or int32")
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def quantize(x, *, tile=False, transpose=False):
@@ -196,25 +214,111 @@ def block_matmul(a, b, bias=None, activation=None, threshold=None, *, out_dtype=
         raise ValueError("jumprelu needs a threshold")
     if activation != "jumprelu":
         threshold = None
-    vectors = []
-    for name, v in (("bias", bias), ("threshold", threshold)):
-        if v is not None:
-            if tuple(v.shape) != (N,) or v.device != dev:
-                raise ValueError(f"{name} must be [{N}] on {dev}, got {list(v.shape)} on {v.device}")
-            _abi.dtype_code(v.dtype, name)
-            v = v.detach().to(torch.float32).contiguous()
-        vectors.append(v)
+    bias = _vector(bias, "bias", N, dev)
+    threshold = _vector(threshold, "threshold", N, dev)
     if out is None:
         _abi.dtype_code(out_dtype, "out_dtype")
         out = torch.empty(M, N, dtype=out_dtype, device=dev)
     elif tuple(out.shape) != (M, N) or out.device != dev:
         raise ValueError(f"out must be {[M, N]} on {dev}, got {list(out.shape)} on {out.device}")
-    m = _abi.matrix(out, "out")
-    lib = _abi.load()
-    need = ctypes.c_size_t(0)
-    _abi.check(lib.sf_block_matmul_workspace(a._ref, b._ref, ctypes.byref(m), ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-    _run(dev, lib.sf_block_matmul, a._ref, b._ref, *(v.data_ptr() if v is not None else None for v in vectors),
-         -1 if activation is None else ACTIVATIONS[activation], ctypes.byref(m),
-         ws.data_ptr() if ws is not None else None, need.value)
+    _product(dev, a._ref, b._ref, bias, threshold, -1 if activation is None else ACTIVATIONS[activation], out)
     return out
+
+
+def _vector(v, name, n, dev):
+    """A [n] vector in contiguous fp32, or None."""
+    if v is None:
+        return None
+    if tuple(v.shape) != (n,) or v.device != dev:
+        raise ValueError(f"{name} must be [{n}] on {dev}, got {list(v.shape)} on {v.device}")
+    if v.dtype != torch.float32:
+        _abi.dtype_code(v.dtype, name)
+        v = v.detach().to(torch.float32)
+    return v if v.is_contiguous() else v.detach().contiguous()
+
+
+def _product(dev, a, b, bias, threshold, activation, out):
+    """sf_block_matmul on ctypes references, with its workspace."""
+    lib = _abi.load()
+    m = ctypes.byref(_abi.matrix(out, "out"))
+    need = ctypes.c_size_t(0)
+    _abi.check(lib.sf_block_matmul_workspace(a, b, m, ctypes.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+    _run(dev, lib.sf_block_matmul, a, b, bias.data_ptr() if bias is not None else None,
+         threshold.data_ptr() if threshold is not None else None, activation, m,
+         ws.data_ptr() if need.value else None, need.value)
+
+
+class _Carver:
+    """Uninitialised BlockScaled structures in one buffer (a step needs up to four: one allocation, no views).
+    Add them, then place() the buffer; the structures are valid while it lives."""
+
+    __slots__ = ("parts", "bytes")
+
+    def __init__(self):
+        self.parts, self.bytes = [], 0
+
+    def add(self, rows, cols, tile):
+        dp, sp, scale_rows, size = _layout(rows, cols, tile)
+        c = _abi.SfBlocks(self.bytes, self.bytes + _cdiv(rows * dp, 256) * 256, rows, cols, dp, sp, int(tile), 0)
+        self.parts.append(c)
+        self.bytes += size
+        return c
+
+    def place(self, dev, buffer=None):
+        if buffer is None:
+            buffer = torch.empty(max(self.bytes, 1), dtype=torch.uint8, device=dev)
+        at = buffer.data_ptr()
+        for c in self.parts:
+            c.data = at + (c.data or 0)
+            c.scales = at + (c.scales or 0)
+        return buffer
+
+
+def linear8_forward(x, W, b, need_x, need_W):
+    """(y, buffer) of saeflow_b200.training.linear8: y = Q(x) @ Q(W) + b in x's dtype, and what its backward
+    reads: Q(x^T) where W needs a gradient, then Q(W) where x does (linear8_backward lays them out alike)."""
+    dev = _abi.require_cuda(("x", x), ("W", W), ("b", b))
+    (M, K), N = x.shape, W.shape[1]
+    xm, wm = _abi.matrix(x, "x"), _abi.matrix(W, "W")
+    bias = _vector(b, "b", N, dev)
+    keep, temp = _Carver(), _Carver()
+    xt = keep.add(K, M, False) if need_W else None
+    wq = keep.add(K, N, True) if need_x else None
+    xq, wt = temp.add(M, K, False), temp.add(N, K, True)
+    kept, used = keep.place(dev) if need_W or need_x else None, temp.place(dev)
+    lib = _abi.load()
+    _run(dev, lib.sf_blocks_quantize, ctypes.byref(xm), ctypes.byref(xq), _abi.ref(xt), None, None, 0)
+    _run(dev, lib.sf_blocks_quantize, ctypes.byref(wm), _abi.ref(wq), ctypes.byref(wt), None, None, 0)
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    _product(dev, ctypes.byref(xq), ctypes.byref(wt), bias, None, -1, y)
+    del used  # stream-ordered: the allocator reuses it after these kernels
+    return y, kept
+
+
+def linear8_backward(dy, kept, M, K, N, x_dtype, W_dtype, need_x, need_W, need_b):
+    """(dx, dW, fp32 db) of linear8 from dy [M, N] and its forward's buffer; None where not needed. M > 0."""
+    dev = _abi.require_cuda(("dy", dy))
+    dm = _abi.matrix(dy, "dy")
+    keep, temp = _Carver(), _Carver()
+    xt = keep.add(K, M, False) if need_W else None
+    wq = keep.add(K, N, True) if need_x else None
+    if kept is not None:
+        keep.place(dev, kept)
+    dyq = temp.add(M, N, False) if need_x or not need_W else None
+    dyt = temp.add(N, M, False) if need_W else None
+    sums_at = temp.bytes
+    n = 4 * _cdiv(M, BLOCK) * N if need_b else 0
+    temp.bytes += n
+    used = temp.place(dev)
+    db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
+    _run(dev, _abi.load().sf_blocks_quantize, ctypes.byref(dm), _abi.ref(dyq), _abi.ref(dyt),
+         db.data_ptr() if need_b else None, used.data_ptr() + sums_at if need_b else None, n)
+    dx = dW = None
+    if need_x:
+        dx = torch.empty(M, K, dtype=x_dtype, device=dev)
+        _product(dev, ctypes.byref(dyq), ctypes.byref(wq), None, None, -1, dx)
+    if need_W:
+        dW = torch.empty(K, N, dtype=W_dtype, device=dev)
+        _product(dev, ctypes.byref(xt), ctypes.byref(dyt), None, None, -1, dW)
+    return dx, dW, db

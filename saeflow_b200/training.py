@@ -30,7 +30,7 @@ import torch
 
 from .kernels import sparse_decode
 from .kernels.backward import csc_gather, csr_sddmm, csr_transpose, matvec, transpose
-from .kernels.blocks import BlockScaled, block_matmul, quantize_both
+from .kernels.blocks import linear8_backward, linear8_forward
 
 
 @dataclass
@@ -105,34 +105,22 @@ def forward(sae, x):
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b):
-        need_x, need_W = ctx.needs_input_grad[:2]
-        xq, xt, _ = quantize_both(x.detach(), want=(True, need_W))
-        wq, wt, _ = quantize_both(W.detach(), tile=True, want=(need_x, True))
-        # two tensors each for what the backward reads: autograd keeps and frees them
-        ctx.save_for_backward(*(t for m in (xt, wq) if m is not None for t in (m.data, m.scales)))
-        ctx.dtypes = x.dtype, W.dtype, None if b is None else b.dtype
-        ctx.shapes = x.shape, W.shape
-        return block_matmul(xq, wt, b, out_dtype=x.dtype)
+        y, kept = linear8_forward(x, W, b, *ctx.needs_input_grad[:2])
+        ctx.save_for_backward(kept)
+        ctx.args = (*x.shape, W.shape[1], x.dtype, W.dtype)
+        ctx.b_dtype = None if b is None else b.dtype
+        return y
 
     @staticmethod
     def backward(ctx, dy):
-        need_x, need_W, need_b = ctx.needs_input_grad[:3]
-        saved = list(ctx.saved_tensors)
-        xt = BlockScaled(saved.pop(0), saved.pop(0)) if need_W else None
-        wq = BlockScaled(saved.pop(0), saved.pop(0), tile=True) if need_x else None
-        x_dtype, W_dtype, b_dtype = ctx.dtypes
-        dx = dW = db = None
-        if not dy.shape[0]:
-            (x_shape, W_shape) = ctx.shapes
-            dx = dy.new_zeros(x_shape, dtype=x_dtype) if need_x else None
-            dW = dy.new_zeros(W_shape, dtype=W_dtype) if need_W else None
-            return dx, dW, dy.new_zeros(dy.shape[1], dtype=b_dtype) if need_b else None
-        if need_x or need_W or need_b:
-            dyq, dyt, sums = quantize_both(dy, want=(need_x or not need_W, need_W), col_sums=need_b)
-            dx = block_matmul(dyq, wq, out_dtype=x_dtype) if need_x else None
-            dW = block_matmul(xt, dyt, out_dtype=W_dtype) if need_W else None
-            db = sums.to(b_dtype) if need_b else None
-        return dx, dW, db
+        needs = ctx.needs_input_grad[:3]
+        M, K, N, x_dtype, W_dtype = ctx.args
+        if not M:
+            return (dy.new_zeros(M, K, dtype=x_dtype) if needs[0] else None,
+                    dy.new_zeros(K, N, dtype=W_dtype) if needs[1] else None,
+                    dy.new_zeros(N, dtype=ctx.b_dtype) if needs[2] else None)
+        dx, dW, db = linear8_backward(dy, ctx.saved_tensors[0], *ctx.args, *needs)
+        return dx, dW, db if db is None or ctx.b_dtype == torch.float32 else db.to(ctx.b_dtype)
 
 
 def linear8(x, W, b=None):
