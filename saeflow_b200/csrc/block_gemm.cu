@@ -17,10 +17,8 @@
 //
 // Two sizes. PAIR: a CTA pair (cta_group::2) computes 256 x 256, each CTA loading 128 rows of either
 // operand; both CTAs' loads complete on the leader's barriers. Single: one CTA computes 128 x COLS.
-// Two orientations. The rows of a tile (TMEM lanes) are rows of `a` and its columns rows of `b`; or,
-// SWAP, the other way round: then a warp's store is 32 neighbouring elements of one output row, which
-// suits outputs whose rows TMA cannot address, and few rows of `a` make a narrow tile (COLS = 32) beside
-// 128 rows of weights.
+// A pair's tile has rows of `a` for its rows (TMEM lanes); a single CTA's has rows of `b`, so that few rows of
+// `a` make a narrow tile (COLS = 32) beside 128 rows of weights.
 #include <algorithm>
 #include <type_traits>
 
@@ -40,7 +38,7 @@ constexpr int kPairCols = 256;                 // columns of a pair's tile
 constexpr int kRowTile = 128;                  // rows (TMEM lanes) per CTA
 
 struct GemmParams {
-    int rows, cols;            // of the tile grid: a's and b's, or b's and a's with SWAP
+    int rows, cols;            // of the tile grid: a's and b's, or b's and a's (kSwapped)
     int nkb, groups;           // K blocks of 128, and groups of four of them
     int splits, split_groups;  // ranges of K: split z takes groups [z split_groups, (z + 1) split_groups)
     int row_tiles, col_tiles;
@@ -52,7 +50,7 @@ struct GemmParams {
     int r_shift, c_shift;      // log2 of the rows a scale row serves: 0 row blocks, 7 tiles
     const float *bias, *thr;
     int activation;            // enum sf_activation, -1 none
-    void *out;                 // SWAP: plain stores
+    void *out;                 // of plain stores
     int64_t out_pitch;
     int64_t out_split;         // elements between the splits' outputs
     unsigned *err;
@@ -76,6 +74,16 @@ struct Shape {
     static constexpr int SCALE_COL = ACC1 + COLS;
     static_assert(SCALE_COL + kScaleSlots * SLOT_COLS <= kTmemCols, "TMEM columns");
 };
+
+// How a tile's sums reach the output. kTma: 32 x 32 boxes, for rows that start on 16-byte boundaries. kRows:
+// 256-byte runs of a row through shared memory, shifted to the output's own 16-byte boundaries. kSwapped: the
+// rows of the tile are the columns of the output, and a warp stores 32 neighbours of one row at a time.
+enum Store { kTma = 0, kRows = 1, kSwapped = 2 };
+
+template <typename OT>
+constexpr int out_bytes(int store) {  // of shared memory per epilogue warp
+    return store == kTma ? 32 * 32 * (int)sizeof(OT) : store == kRows ? 32 * 256 : 0;
+}
 
 struct __align__(16) Shared {
     uint64_t full[12], empty[12];
@@ -123,6 +131,75 @@ __device__ __forceinline__ uint4 scale_words(const uint8_t *s, int64_t pitch, in
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Two neighbours in the output type, or one fp32 word each: 16-bit conversions in pairs (one by one they run
+// at a quarter of the rate, and took half of the epilogue).
+template <typename OT>
+__device__ __forceinline__ void pack32(const float (&v)[32], uint32_t (&o)[8 * sizeof(OT)]) {
+    if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
+    } else if constexpr (std::is_same_v<OT, __nv_bfloat16>) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            o[j] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            o[j] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    }
+}
+
+// 256 bytes of each of 32 output rows from a warp's buffer (16-byte chunk j of row r at chunk j ^ r % 16) to
+// `out`, the first row's run; the runs start between 16-byte boundaries, each at its own place. A half warp
+// takes a row: the aligned chunks by shifting two of the buffer's into one, then the elements before the
+// first and after the last boundary, a lane to a row. `rows` and `cols` of them exist.
+template <typename OT>
+__device__ __forceinline__ void store_runs(const uint8_t *buf, OT *out, int64_t pitch, int rows, int cols, int lane) {
+    constexpr int E = 16 / sizeof(OT), ES = sizeof(OT);
+    const int limit = min(cols, 16 * E);
+    auto lead_of = [&](int r) {  // elements before the first boundary
+        return (int)((0u - (uint32_t)reinterpret_cast<uintptr_t>(out + r * pitch)) & 15u) / ES;
+    };
+#pragma unroll 4
+    for (int it = 0; it < 16; ++it) {
+        const int r = 2 * it + (lane >> 4), d = lane & 15;
+        const int lead = lead_of(r);
+        if (r >= rows || lead + E * (d + 1) > limit) continue;
+        const uint4 a = *reinterpret_cast<const uint4 *>(buf + r * 256 + ((d ^ (r & 15)) << 4));
+        uint4 b = a;
+        if (lead) b = *reinterpret_cast<const uint4 *>(buf + r * 256 + (((d + 1) ^ (r & 15)) << 4));
+        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const int bytes = lead * ES;
+#pragma unroll
+        for (int j = 0; j < 6; ++j) w[j] = (bytes & 8) ? w[j + 2] : w[j];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) w[j] = (bytes & 4) ? w[j + 1] : w[j];
+        if (ES == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = (bytes & 2) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+        }
+        *reinterpret_cast<uint4 *>(out + r * pitch + lead + E * d) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (lane < rows) {
+        const int lead = lead_of(lane);
+        const int tail = lead + max(0, limit - lead) / E * E;  // the first element after the last boundary
+        OT *dst = out + lane * pitch;
+        auto one = [&](int j) {
+            const int at = j * ES;
+            dst[j] = *reinterpret_cast<const OT *>(buf + lane * 256 + (((at >> 4) ^ (lane & 15)) << 4) + (at & 15));
+        };
+#pragma unroll
+        for (int j = 0; j < E - 1; ++j) {
+            if (j < min(lead, limit)) one(j);
+            if (tail + j < limit) one(tail + j);
+        }
+    }
+}
+
 // max(v, floor) that keeps a NaN (fmaxf would drop it): ReLU with floor 0, nothing with floor -inf.
 __device__ __forceinline__ float at_least(float v, float floor) {
     float r;
@@ -152,18 +229,18 @@ __device__ __forceinline__ void finish_columns(const uint32_t (&r)[32], const fl
     }
 }
 
-template <typename OT, typename S, bool SWAP>
+template <typename OT, typename S, int STORE>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_kernel(const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmC,
                       const __grid_constant__ CUtensorMap tmOut, const GemmParams p) {
-    constexpr bool PAIR = S::PAIR;
+    constexpr bool PAIR = S::PAIR, SWAP = STORE == kSwapped;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sR = smem;
     uint8_t *sC = sR + S::STAGES * S::R_BYTES;
-    constexpr int OUT_BYTES = 32 * 32 * sizeof(OT);
-    uint8_t *sOut = sC + S::STAGES * S::C_BYTES;  // one buffer per epilogue warp (not with SWAP)
-    uint8_t *sScale = sOut + (SWAP ? 0 : kEpilogueWarps * OUT_BYTES);
+    constexpr int OUT_BYTES = out_bytes<OT>(STORE);
+    uint8_t *sOut = sC + S::STAGES * S::C_BYTES;  // one buffer per epilogue warp
+    uint8_t *sScale = sOut + kEpilogueWarps * OUT_BYTES;
     Shared *sh = reinterpret_cast<Shared *>(sScale + kScaleSlots * S::SLOT_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -191,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_mbar_init();
         tma_prefetch_desc(&tmR);
         tma_prefetch_desc(&tmC);
-        if (!SWAP) tma_prefetch_desc(&tmOut);
+        if (STORE == kTma) tma_prefetch_desc(&tmOut);
     }
     if (warp == 1) {
         if (PAIR) {
@@ -386,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float floor = floor_of(p.activation);
         int acc = 0;
         uint32_t acc_phase = 0;
-        // This thread's bias and threshold of the coming tile, loaded a tile ahead: its row's with SWAP, else
+        // This thread's bias and threshold of the coming tile, loaded a tile ahead: its row's (kSwapped), else
         // column et's, for shared memory.
         static_assert(SWAP || S::COLS == 32 * kEpilogueWarps, "a column to each epilogue thread");
         float next_bias, next_thr;
@@ -433,41 +510,67 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int h = 0; h < STEP / 32; ++h) {
                     const int c = c0 + 32 * h;
+                    float v[32];
+                    uint32_t o[8 * sizeof(OT)];
                     if constexpr (SWAP) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = at_least(__uint_as_float(r[h][j]) + row_bias, floor);
+                        if (p.thr) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = jump(v[j], row_thr);
+                        }
+                        pack32<OT>(v, o);
                         if (row < p.rows) {
                             OT *dst = reinterpret_cast<OT *>(p.out) + un.split * p.out_split +
                                       (int64_t)(un.col0 + c) * p.out_pitch + row;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                float v = at_least(__uint_as_float(r[h][j]) + row_bias, floor);
-                                if (p.thr) v = jump(v, row_thr);
-                                if (un.col0 + c + j < p.cols) dst[j * p.out_pitch] = from_f32<OT>(v);
-                            }
+                            for (int j = 0; j < 32; ++j)
+                                if (un.col0 + c + j < p.cols)
+                                    dst[j * p.out_pitch] = reinterpret_cast<const OT *>(o)[j];
                         }
                     } else {
-                        float v[32];
                         finish_columns(r[h], sh->bias[acc] + c, p.thr ? sh->thr[acc] + c : nullptr, floor, v);
-                        alignas(16) OT o[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = from_f32<OT>(v[j]);
+                        pack32<OT>(v, o);
                         uint8_t *buf = sOut + (warp - 2) * OUT_BYTES;
-                        tma_store_wait_read<0>();  // the last store has read the buffer
-                        __syncwarp();
-                        // 32 rows of 32 columns, 16-byte chunks swizzled as the tensor map says: 128-byte rows of fp32
-                        // (chunk ^ row % 8), 64-byte rows of 16-bit outputs (chunk ^ row / 2 % 4)
-                        constexpr int CHUNKS = 2 * sizeof(OT);
-                        const int swz = sizeof(OT) == 4 ? lane & 7 : (lane >> 1) & 3;
-#pragma unroll
-                        for (int j = 0; j < CHUNKS; ++j)
-                            *reinterpret_cast<uint4 *>(buf + lane * (16 * CHUNKS) + ((j ^ swz) << 4)) =
-                                reinterpret_cast<const uint4 *>(o)[j];
-                        fence_proxy_async_smem();
-                        __syncwarp();
                         const int row_w = un.row0 + (int)rank * kRowTile + quad * 32;
-                        if (lane == 0) {
-                            if (row_w < p.rows && un.col0 + c < p.cols)
-                                tma_store_3d(&tmOut, buf, un.col0 + c, row_w, un.split);
-                            tma_store_commit();
+                        constexpr int CHUNKS = 2 * sizeof(OT);
+                        if constexpr (STORE == kTma) {
+                            tma_store_wait_read<0>();  // the last store has read the buffer
+                            __syncwarp();
+                            // 32 rows of 32 columns, 16-byte chunks swizzled as the tensor map says: 128-byte rows of
+                            // fp32 (chunk ^ row % 8), 64-byte rows of 16-bit outputs (chunk ^ row / 2 % 4)
+                            const int swz = sizeof(OT) == 4 ? lane & 7 : (lane >> 1) & 3;
+#pragma unroll
+                            for (int j = 0; j < CHUNKS; ++j)
+                                *reinterpret_cast<uint4 *>(buf + lane * (16 * CHUNKS) + ((j ^ swz) << 4)) =
+                                    make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (row_w < p.rows && un.col0 + c < p.cols)
+                                    tma_store_3d(&tmOut, buf, un.col0 + c, row_w, un.split);
+                                tma_store_commit();
+                            }
+                        } else {
+                            // 256 bytes of a row: this warp's 128 columns of 16 bits, or 64 of fp32
+                            constexpr int RUN = 256 / sizeof(OT);
+                            const int c_run = c / RUN * RUN;
+#pragma unroll
+                            for (int j = 0; j < CHUNKS; ++j) {
+                                const int chunk = (c - c_run) * (int)sizeof(OT) / 16 + j;
+                                *reinterpret_cast<uint4 *>(buf + lane * 256 + ((chunk ^ (lane & 15)) << 4)) =
+                                    make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                            }
+                            if (h == STEP / 32 - 1 && (sizeof(OT) == 4 || i == my_steps - 1)) {
+                                __syncwarp();
+                                const int n = p.cols - un.col0 - c_run;
+                                if (n > 0 && row_w < p.rows)
+                                    store_runs<OT>(buf,
+                                                   reinterpret_cast<OT *>(p.out) + un.split * p.out_split +
+                                                       (int64_t)row_w * p.out_pitch + un.col0 + c_run,
+                                                   p.out_pitch, p.rows - row_w, n, lane);
+                                __syncwarp();
+                            }
                         }
                     }
                 }
@@ -477,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 acc_phase ^= 1u;
             }
         }
-        if (!SWAP) tma_store_wait_read<0>();  // the buffers go with the CTA
+        if (STORE == kTma) tma_store_wait_read<0>();  // the buffers go with the CTA
     } else {
         // ---------------------------------------------------------------- scales (both CTAs)
         // A group's words are loaded while the one before waits for its slot: a load from HBM takes as long
@@ -568,11 +671,11 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const float *__restric
 
 // ------------------------------------------------------------------------------- host side
 
-template <typename OT, typename S, bool SWAP>
+template <typename OT, typename S, int STORE>
 int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tmOut, const GemmParams &p,
            cudaStream_t stream) {
-    auto kern = block_gemm_kernel<OT, S, SWAP>;
-    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + (SWAP ? 0 : kEpilogueWarps * 32 * 32 * sizeof(OT)) +
+    auto kern = block_gemm_kernel<OT, S, STORE>;
+    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + kEpilogueWarps * out_bytes<OT>(STORE) +
                             kScaleSlots * S::SLOT_BYTES + sizeof(Shared);
     static_assert(smem <= 232448, "shared memory per block");
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -600,22 +703,23 @@ int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tm
     return check_cuda(cudaGetLastError(), "block_gemm launch");
 }
 
-using Pair16 = Shape<true, kPairCols, 6>;  // 16-bit outputs, or SWAP
-using Pair32 = Shape<true, kPairCols, 5>;  // fp32 outputs: larger store buffers
+// Operand stages: what the store buffers leave of shared memory.
+template <typename OT, int STORE>
+using Pair = Shape<true, kPairCols, STORE == kRows ? 4 : sizeof(OT) == 4 ? 5 : 6>;
 using One32 = Shape<false, 32, 10>;
 using One64 = Shape<false, 64, 8>;
 using One128 = Shape<false, 128, 6>;
 
 // What a call does, from its sizes alone.
 struct Plan {
-    bool pair, swap;
-    int cols;    // columns of a tile
+    bool pair;   // CTA pairs on 256 x 256 tiles; else single CTAs on 128 rows of b x `cols` rows of a (kSwapped)
+    int cols;
     int splits;  // ranges of K
 };
 
 int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-Plan make_plan(int64_t M, int64_t N, int64_t K, bool tma_out, int out_dtype) {
+Plan make_plan(int64_t M, int64_t N, int64_t K, int out_dtype) {
     Plan pl{};
     const int sms = num_sms();
     const int groups = cdiv(K, 4 * kKBytes);
@@ -623,10 +727,9 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool tma_out, int out_dtype) {
     // CTA (a pair's CTA loads half of its columns), and a pair's tile is twice the work per CTA.
     const int cols = M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const int64_t one_tiles = (int64_t)cdiv(N, 128) * cdiv(M, cols);
-    const int64_t pair_tiles = tma_out ? (int64_t)cdiv(N, kPairCols) * cdiv(M, 256) : (int64_t)cdiv(N, 256) * cdiv(M, kPairCols);
+    const int64_t pair_tiles = (int64_t)cdiv(N, 256) * cdiv(M, 256);
     const int64_t one_cost = cdiv(one_tiles, sms) * (int64_t)(128 + cols), pair_cost = cdiv(pair_tiles, sms / 2) * 256;
     pl.pair = M > 128 && pair_cost < one_cost;
-    pl.swap = !pl.pair || !tma_out;
     pl.cols = pl.pair ? kPairCols : cols;
     const int64_t tiles = pl.pair ? pair_tiles : one_tiles;
     const int slots = pl.pair ? sms / 2 : sms;
@@ -669,13 +772,14 @@ bool tma_rows(const sf_matrix &out) {
 }
 
 template <typename OT>
-int run_plan(const Plan &pl, const CUtensorMap &r, const CUtensorMap &c, const CUtensorMap &o, const GemmParams &p,
+int run_plan(const Plan &pl, int store, const CUtensorMap &r, const CUtensorMap &c, const CUtensorMap &o, const GemmParams &p,
              cudaStream_t s) {
-    using Pair = std::conditional_t<sizeof(OT) == 4, Pair32, Pair16>;
-    if (pl.pair) return pl.swap ? launch<OT, Pair16, true>(r, c, o, p, s) : launch<OT, Pair, false>(r, c, o, p, s);
-    if (pl.cols == 32) return launch<OT, One32, true>(r, c, o, p, s);
-    if (pl.cols == 64) return launch<OT, One64, true>(r, c, o, p, s);
-    return launch<OT, One128, true>(r, c, o, p, s);
+    if (pl.pair)
+        return store == kTma ? launch<OT, Pair<OT, kTma>, kTma>(r, c, o, p, s)
+                             : launch<OT, Pair<OT, kRows>, kRows>(r, c, o, p, s);
+    if (pl.cols == 32) return launch<OT, One32, kSwapped>(r, c, o, p, s);
+    if (pl.cols == 64) return launch<OT, One64, kSwapped>(r, c, o, p, s);
+    return launch<OT, One128, kSwapped>(r, c, o, p, s);
 }
 
 }  // namespace
@@ -692,7 +796,7 @@ int sf_block_matmul_workspace(const sf_blocks *a, const sf_blocks *b, const sf_m
     if (!bytes) return set_error(SF_ERR_INVALID, "bytes is NULL");
     *bytes = 0;
     if (out->rows == 0 || out->cols == 0) return SF_OK;
-    const Plan pl = make_plan(a->rows, b->rows, a->cols, tma_rows(*out), out->dtype);
+    const Plan pl = make_plan(a->rows, b->rows, a->cols, out->dtype);
     if (pl.splits > 1) *bytes = (size_t)pl.splits * out->rows * partial_pitch(out->cols) * sizeof(float);
     return SF_OK;
 }
@@ -709,7 +813,7 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
         return set_error(SF_ERR_WORKSPACE, "16-byte aligned workspace of %zu bytes needed", need);
     const int M = (int)a->rows, N = (int)b->rows;
-    const Plan pl = make_plan(M, N, a->cols, tma_rows(*out), out->dtype);
+    const Plan pl = make_plan(M, N, a->cols, out->dtype);
     if ((int64_t)cdiv(M, 32) * cdiv(N, 128) * pl.splits > INT32_MAX / 2)
         return set_error(SF_ERR_UNSUPPORTED, "too many output tiles and ranges of K");
     // Partial sums go to the workspace in fp32, without bias or activation, and are joined after.
@@ -720,7 +824,8 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
         dst.dtype = SF_F32;
         dst.stride_row = partial_pitch(N);
     }
-    const sf_blocks *R = pl.swap ? b : a, *C = pl.swap ? a : b;
+    const int store = !pl.pair ? kSwapped : tma_rows(dst) ? kTma : kRows;
+    const sf_blocks *R = pl.pair ? a : b, *C = pl.pair ? b : a;
     const int row_tile = pl.pair ? 256 : 128;
     GemmParams p{};
     p.rows = (int)R->rows;
@@ -761,17 +866,17 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     if ((st = make_map_e4m3(&tmC, C->data, (uint64_t)C->cols, (uint64_t)C->rows, (uint64_t)C->data_pitch, box)))
         return st;
     const int64_t es = (int64_t)dtype_size(dst.dtype);
-    if (!pl.swap &&
+    if (store == kTma &&
         (st = make_map_out(&tmOut, dst.data, dst.dtype, (uint64_t)N, (uint64_t)M, (uint64_t)pl.splits,
                            (uint64_t)(dst.stride_row * es), (uint64_t)(p.out_split * es))))
         return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (dst.dtype == SF_BF16)
-        st = run_plan<__nv_bfloat16>(pl, tmR, tmC, tmOut, p, s);
+        st = run_plan<__nv_bfloat16>(pl, store, tmR, tmC, tmOut, p, s);
     else if (dst.dtype == SF_F16)
-        st = run_plan<__half>(pl, tmR, tmC, tmOut, p, s);
+        st = run_plan<__half>(pl, store, tmR, tmC, tmOut, p, s);
     else
-        st = run_plan<float>(pl, tmR, tmC, tmOut, p, s);
+        st = run_plan<float>(pl, store, tmR, tmC, tmOut, p, s);
     if (st || !partial) return st;
     const dim3 grid(cdiv(N, 1024), std::min(M, 65535));
     const float *part = static_cast<const float *>(workspace);
