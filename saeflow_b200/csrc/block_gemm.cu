@@ -75,14 +75,13 @@ struct Shape {
     static_assert(SCALE_COL + kScaleSlots * SLOT_COLS <= kTmemCols, "TMEM columns");
 };
 
-// How a tile's sums reach the output. kTma: 32 x 32 boxes, for rows that start on 16-byte boundaries. kRows:
+// How a tile's sums reach the output. kTma: boxes of 32 rows x 128 bytes, for rows that start on 16-byte boundaries. kRows:
 // 256-byte runs of a row through shared memory, shifted to the output's own 16-byte boundaries. kSwapped: the
 // rows of the tile are the columns of the output, and a warp stores 32 neighbours of one row at a time.
 enum Store { kTma = 0, kRows = 1, kSwapped = 2 };
 
-template <typename OT>
 constexpr int out_bytes(int store) {  // of shared memory per epilogue warp
-    return store == kTma ? 32 * 32 * (int)sizeof(OT) : store == kRows ? 32 * 256 : 0;
+    return store == kTma ? 32 * 128 : store == kRows ? 32 * 256 : 0;
 }
 
 struct __align__(16) Shared {
@@ -92,8 +91,8 @@ struct __align__(16) Shared {
     uint64_t drain;
     uint32_t tmem_base;
     int abort_flag;
-    alignas(16) float bias[2][256];
-    alignas(16) float thr[2][256];
+    alignas(16) float bias[kEpilogueWarps][128];
+    alignas(16) float thr[kEpilogueWarps][128];
 };
 
 struct Unit {
@@ -131,25 +130,85 @@ __device__ __forceinline__ uint4 scale_words(const uint8_t *s, int64_t pitch, in
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Two neighbours in the output type, or one fp32 word each: 16-bit conversions in pairs (one by one they run
-// at a quarter of the rate, and took half of the epilogue).
+// max(v, floor) that keeps a NaN (fmaxf would drop it): ReLU with floor 0, nothing with floor -inf.
+__device__ __forceinline__ float at_least(float v, float floor) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(floor));
+    return r;
+}
+__device__ __forceinline__ float jump(float v, float t) { return v > t && v > 0.f ? v : 0.f; }
+__device__ __forceinline__ float floor_of(int activation) {
+    return activation == SF_ACT_RELU ? 0.f : __int_as_float(0xff800000);
+}
+
+// max of two 16-bit floats each and zero, keeping NaN.
 template <typename OT>
-__device__ __forceinline__ void pack32(const float (&v)[32], uint32_t (&o)[8 * sizeof(OT)]) {
+__device__ __forceinline__ uint32_t relu2(uint32_t w) {
+    uint32_t r;
+    if constexpr (std::is_same_v<OT, __nv_bfloat16>)
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+    else
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+    return r;
+}
+
+// Two neighbours in a 16-bit output type (converted one by one they run at a quarter of the rate).
+template <typename OT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same_v<OT, __nv_bfloat16>) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// Bias, activation and rounding of 32 sums: the words of the output. `bias(j)` gives four at a time, `thr(j)` one.
+// The activation is uniform: tested once, not per element (which took 1350 clocks). ReLU of a 16-bit output
+// comes after its rounding, two at a time; both are monotone, so their order does not matter.
+template <typename OT, typename Bias, typename Thr>
+__device__ __forceinline__ void finish32(uint32_t (&r)[32], int activation, Bias bias, Thr thr,
+                                         uint32_t (&o)[8 * sizeof(OT)]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 b = bias(j);
+        r[j] = __float_as_uint(__uint_as_float(r[j]) + b.x);
+        r[j + 1] = __float_as_uint(__uint_as_float(r[j + 1]) + b.y);
+        r[j + 2] = __float_as_uint(__uint_as_float(r[j + 2]) + b.z);
+        r[j + 3] = __float_as_uint(__uint_as_float(r[j + 3]) + b.w);
+    }
+    if (activation == SF_ACT_JUMPRELU) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(jump(__uint_as_float(r[j]), thr(j)));
+    }
     if constexpr (sizeof(OT) == 4) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
-    } else if constexpr (std::is_same_v<OT, __nv_bfloat16>) {
+        for (int j = 0; j < 32; ++j) o[j] = r[j];
+        if (activation == SF_ACT_RELU) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            o[j] = *reinterpret_cast<const uint32_t *>(&h);
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(at_least(__uint_as_float(o[j]), 0.f));
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            o[j] = *reinterpret_cast<const uint32_t *>(&h);
+        for (int j = 0; j < 16; ++j) o[j] = pack2<OT>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+        if (activation == SF_ACT_RELU) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = relu2<OT>(o[j]);
         }
+    }
+}
+
+// Eight words shifted right by `bytes` < 16, a multiple of 2 (of 4 where ES is 4): the first four.
+template <int ES>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[8], int bytes) {
+#pragma unroll
+    for (int j = 0; j < 6; ++j) w[j] = (bytes & 8) ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = (bytes & 4) ? w[j + 1] : w[j];
+    if (ES == 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = (bytes & 2) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
     }
 }
 
@@ -173,59 +232,60 @@ __device__ __forceinline__ void store_runs(const uint8_t *buf, OT *out, int64_t 
         uint4 b = a;
         if (lead) b = *reinterpret_cast<const uint4 *>(buf + r * 256 + (((d + 1) ^ (r & 15)) << 4));
         uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        const int bytes = lead * ES;
-#pragma unroll
-        for (int j = 0; j < 6; ++j) w[j] = (bytes & 8) ? w[j + 2] : w[j];
-#pragma unroll
-        for (int j = 0; j < 5; ++j) w[j] = (bytes & 4) ? w[j + 1] : w[j];
-        if (ES == 2) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = (bytes & 2) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
-        }
+        shift_words<ES>(w, lead * ES);
         *reinterpret_cast<uint4 *>(out + r * pitch + lead + E * d) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (lane < rows) {
-        const int lead = lead_of(lane);
-        const int tail = lead + max(0, limit - lead) / E * E;  // the first element after the last boundary
-        OT *dst = out + lane * pitch;
-        auto one = [&](int j) {
-            const int at = j * ES;
-            dst[j] = *reinterpret_cast<const OT *>(buf + lane * 256 + (((at >> 4) ^ (lane & 15)) << 4) + (at & 15));
-        };
+    if (lane >= rows) return;
+    const int lead = lead_of(lane);
+    OT *dst = out + lane * pitch;
+    if (limit == 16 * E) {
+        // Whole runs: the first `lead` elements and the last E - lead, as pieces of 2, 4 and 8 bytes that end and
+        // start at a boundary (element by element they took longer than all the rest).
+        if (lead == 0) return;
+        const uint4 a = *reinterpret_cast<const uint4 *>(buf + lane * 256 + ((lane & 15) << 4));
+        const uint4 b = *reinterpret_cast<const uint4 *>(buf + lane * 256 + ((15 ^ (lane & 15)) << 4));
+        uint32_t w[8] = {a.x, a.y, a.z, a.w, 0u, 0u, 0u, 0u}, t[8] = {b.x, b.y, b.z, b.w, 0u, 0u, 0u, 0u};
+        uint8_t *to = reinterpret_cast<uint8_t *>(dst);
+        int bytes = lead * ES;
+        if (ES == 2 && (bytes & 2)) {
+            *reinterpret_cast<uint16_t *>(to) = (uint16_t)w[0];
+            to += 2;
 #pragma unroll
-        for (int j = 0; j < E - 1; ++j) {
-            if (j < min(lead, limit)) one(j);
-            if (tail + j < limit) one(tail + j);
+            for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
         }
+        if (bytes & 4) {
+            *reinterpret_cast<uint32_t *>(to) = w[0];
+            to += 4;
+            w[0] = w[1];
+            w[1] = w[2];
+        }
+        if (bytes & 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+        shift_words<ES>(t, bytes);
+        to = reinterpret_cast<uint8_t *>(dst + 15 * E + lead);
+        bytes = 16 - bytes;
+        if (bytes & 8) {
+            *reinterpret_cast<uint2 *>(to) = make_uint2(t[0], t[1]);
+            to += 8;
+            t[0] = t[2];
+            t[1] = t[3];
+        }
+        if (bytes & 4) {
+            *reinterpret_cast<uint32_t *>(to) = t[0];
+            to += 4;
+            t[0] = t[1];
+        }
+        if (ES == 2 && (bytes & 2)) *reinterpret_cast<uint16_t *>(to) = (uint16_t)t[0];
+        return;
     }
-}
-
-// max(v, floor) that keeps a NaN (fmaxf would drop it): ReLU with floor 0, nothing with floor -inf.
-__device__ __forceinline__ float at_least(float v, float floor) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(floor));
-    return r;
-}
-__device__ __forceinline__ float jump(float v, float t) { return v > t && v > 0.f ? v : 0.f; }
-__device__ __forceinline__ float floor_of(int activation) {
-    return activation == SF_ACT_RELU ? 0.f : __int_as_float(0xff800000);
-}
-
-// Bias and activation of 32 columns. The activation is uniform: one test per 32 columns, none per element
-// (with a test per element this loop took 1350 clocks, four times the rest of the epilogue).
-__device__ __forceinline__ void finish_columns(const uint32_t (&r)[32], const float *bias, const float *thr,
-                                               float floor, float (&v)[32]) {
+    const int tail = lead + max(0, limit - lead) / E * E;  // the first element after the last boundary
+    auto one = [&](int j) {
+        const int at = j * ES;
+        dst[j] = *reinterpret_cast<const OT *>(buf + lane * 256 + (((at >> 4) ^ (lane & 15)) << 4) + (at & 15));
+    };
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-        const float4 b = *reinterpret_cast<const float4 *>(bias + j);
-        v[j] = at_least(__uint_as_float(r[j]) + b.x, floor);
-        v[j + 1] = at_least(__uint_as_float(r[j + 1]) + b.y, floor);
-        v[j + 2] = at_least(__uint_as_float(r[j + 2]) + b.z, floor);
-        v[j + 3] = at_least(__uint_as_float(r[j + 3]) + b.w, floor);
-    }
-    if (thr) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = jump(v[j], thr[j]);
+    for (int j = 0; j < E - 1; ++j) {
+        if (j < min(lead, limit)) one(j);
+        if (tail + j < limit) one(tail + j);
     }
 }
 
@@ -238,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sR = smem;
     uint8_t *sC = sR + S::STAGES * S::R_BYTES;
-    constexpr int OUT_BYTES = out_bytes<OT>(STORE);
+    constexpr int OUT_BYTES = out_bytes(STORE);
     uint8_t *sOut = sC + S::STAGES * S::C_BYTES;  // one buffer per epilogue warp
     uint8_t *sScale = sOut + kEpilogueWarps * OUT_BYTES;
     Shared *sh = reinterpret_cast<Shared *>(sScale + kScaleSlots * S::SLOT_BYTES);
@@ -452,42 +512,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp < 2 + kEpilogueWarps) {
         // ---------------------------------------------------------------- epilogue
-        const int et = threadIdx.x - 64;
         const int quad = warp & 3;
         // This warp's columns: a half of the tile's, or the first warp all 32 of the narrowest.
         constexpr int HALF = S::COLS < 64 ? S::COLS : S::COLS / 2;
         constexpr int STEP = HALF < 64 ? HALF : 64;  // columns loaded at a time
         constexpr int STEPS = HALF / STEP;
+        static_assert(STEPS <= 2, "at most two steps a tile");
         const int half = (warp - 2) >> 2;
-        const int my_steps = half * HALF < S::COLS ? STEPS : 0;
-        const float floor = floor_of(p.activation);
+        const bool mine = half * HALF < S::COLS;
         int acc = 0;
         uint32_t acc_phase = 0;
-        // This thread's bias and threshold of the coming tile, loaded a tile ahead: its row's (kSwapped), else
-        // column et's, for shared memory.
-        static_assert(SWAP || S::COLS == 32 * kEpilogueWarps, "a column to each epilogue thread");
-        float next_bias, next_thr;
+        // Bias and threshold of the coming tile, loaded a tile ahead: this thread's row's (kSwapped), else those of
+        // this warp's columns, passed through the warp's own shared memory (no barrier between warps).
+        constexpr int OWN = SWAP ? 1 : HALF / 32;
+        float next_bias[OWN], next_thr[OWN];
+        float *my_bias = sh->bias[warp - 2], *my_thr = sh->thr[warp - 2];
         auto load_vectors = [&](int u) {
             const Unit un = unit_of<S>(p, min(u, units - 1));
-            const int at = SWAP ? un.row0 + (int)rank * kRowTile + quad * 32 + lane : un.col0 + et;
-            const bool have = at < (SWAP ? p.rows : p.cols);
-            next_bias = p.bias && have ? __ldg(p.bias + at) : 0.f;
-            next_thr = p.thr && have ? __ldg(p.thr + at) : 0.f;
+#pragma unroll
+            for (int j = 0; j < OWN; ++j) {
+                const int at = SWAP ? un.row0 + (int)rank * kRowTile + quad * 32 + lane
+                                    : un.col0 + half * HALF + 32 * j + lane;
+                const bool have = at < (SWAP ? p.rows : p.cols);
+                next_bias[j] = p.bias && have ? __ldg(p.bias + at) : 0.f;
+                next_thr[j] = p.thr && have ? __ldg(p.thr + at) : 0.f;
+            }
         };
         load_vectors(first_unit);
         for (int u = first_unit; u < units; u += step_units) {
             const Unit un = unit_of<S>(p, u);
             const int row = un.row0 + (int)rank * kRowTile + quad * 32 + lane;
-            const float row_bias = next_bias, row_thr = next_thr;
+            const float row_bias = next_bias[0], row_thr = next_thr[0];
             if (!SWAP) {
-                sh->bias[acc][et] = next_bias;
-                sh->thr[acc][et] = next_thr;
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
+#pragma unroll
+                for (int j = 0; j < OWN; ++j) {
+                    my_bias[32 * j + lane] = next_bias[j];
+                    my_thr[32 * j + lane] = next_thr[j];
+                }
+                __syncwarp();
             }
             load_vectors(u + step_units);
             if (!wait(&sh->tmem_full[acc], acc_phase)) break;
             tc_fence_after();
-            const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1;
+            const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1 + half * HALF;
             // Overlapping accumulators: the shared columns (the first's last 40, the second's first 40) are
             // read first and released to the next tile's MMAs. A warp whose half has none of them releases at
             // once: what it still had to read of the tile before, in the accumulator that those MMAs take, it has.
@@ -497,59 +564,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) arrive_leader(&sh->tmem_empty[acc]);
             };
-            if (!shares || my_steps == 0) release();
-            const int first = S::OVERLAP && acc == 0 ? STEPS - 1 : 0;
-#pragma unroll 1
-            for (int i = 0; i < my_steps; ++i) {
-                const int c0 = half * HALF + (first + i) % STEPS * STEP;
-                uint32_t r[STEP / 32][32];
-#pragma unroll
-                for (int h = 0; h < STEP / 32; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
-                tmem_ld_wait();
-                if (shares && i == (S::OVERLAP ? 0 : STEPS - 1)) release();
+            if (!shares || !mine) release();
+
+            // Columns [c0, c0 + STEP) of this warp's half, from r to the output.
+            auto put = [&](uint32_t (&r)[STEP / 32][32], int c0, bool last) {
 #pragma unroll
                 for (int h = 0; h < STEP / 32; ++h) {
                     const int c = c0 + 32 * h;
-                    float v[32];
+                    const int col = un.col0 + half * HALF + c;
                     uint32_t o[8 * sizeof(OT)];
                     if constexpr (SWAP) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = at_least(__uint_as_float(r[h][j]) + row_bias, floor);
-                        if (p.thr) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = jump(v[j], row_thr);
-                        }
-                        pack32<OT>(v, o);
+                        finish32<OT>(
+                            r[h], p.activation, [&](int) { return make_float4(row_bias, row_bias, row_bias, row_bias); },
+                            [&](int) { return row_thr; }, o);
                         if (row < p.rows) {
                             OT *dst = reinterpret_cast<OT *>(p.out) + un.split * p.out_split +
-                                      (int64_t)(un.col0 + c) * p.out_pitch + row;
+                                      (int64_t)col * p.out_pitch + row;
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (un.col0 + c + j < p.cols)
-                                    dst[j * p.out_pitch] = reinterpret_cast<const OT *>(o)[j];
+                                if (col + j < p.cols) dst[j * p.out_pitch] = reinterpret_cast<const OT *>(o)[j];
                         }
                     } else {
-                        finish_columns(r[h], sh->bias[acc] + c, p.thr ? sh->thr[acc] + c : nullptr, floor, v);
-                        pack32<OT>(v, o);
+                        finish32<OT>(
+                            r[h], p.activation, [&](int j) { return *reinterpret_cast<const float4 *>(my_bias + c + j); },
+                            [&](int j) { return my_thr[c + j]; }, o);
                         uint8_t *buf = sOut + (warp - 2) * OUT_BYTES;
                         const int row_w = un.row0 + (int)rank * kRowTile + quad * 32;
                         constexpr int CHUNKS = 2 * sizeof(OT);
                         if constexpr (STORE == kTma) {
-                            tma_store_wait_read<0>();  // the last store has read the buffer
-                            __syncwarp();
-                            // 32 rows of 32 columns, 16-byte chunks swizzled as the tensor map says: 128-byte rows of
-                            // fp32 (chunk ^ row % 8), 64-byte rows of 16-bit outputs (chunk ^ row / 2 % 4)
-                            const int swz = sizeof(OT) == 4 ? lane & 7 : (lane >> 1) & 3;
+                            // 32 rows of 128 bytes (64 columns of 16 bits, 32 of fp32), 16-byte chunk j of row r at
+                            // chunk j ^ r % 8 as the tensor map says
+                            if (h == 0 || sizeof(OT) == 4) {
+                                tma_store_wait_read<0>();  // the last store has read the buffer
+                                __syncwarp();
+                            }
 #pragma unroll
-                            for (int j = 0; j < CHUNKS; ++j)
-                                *reinterpret_cast<uint4 *>(buf + lane * (16 * CHUNKS) + ((j ^ swz) << 4)) =
+                            for (int j = 0; j < CHUNKS; ++j) {
+                                const int chunk = (sizeof(OT) == 4 ? 0 : CHUNKS * h) + j;
+                                *reinterpret_cast<uint4 *>(buf + lane * 128 + ((chunk ^ (lane & 7)) << 4)) =
                                     make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) {
-                                if (row_w < p.rows && un.col0 + c < p.cols)
-                                    tma_store_3d(&tmOut, buf, un.col0 + c, row_w, un.split);
-                                tma_store_commit();
+                            }
+                            if (h == STEP / 32 - 1 || sizeof(OT) == 4) {
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                                const int col_w = sizeof(OT) == 4 ? col : col - 32 * h;
+                                if (lane == 0) {
+                                    if (row_w < p.rows && col_w < p.cols)
+                                        tma_store_3d(&tmOut, buf, col_w, row_w, un.split);
+                                    tma_store_commit();
+                                }
                             }
                         } else {
                             // 256 bytes of a row: this warp's 128 columns of 16 bits, or 64 of fp32
@@ -561,18 +624,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 *reinterpret_cast<uint4 *>(buf + lane * 256 + ((chunk ^ (lane & 15)) << 4)) =
                                     make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                             }
-                            if (h == STEP / 32 - 1 && (sizeof(OT) == 4 || i == my_steps - 1)) {
+                            if (h == STEP / 32 - 1 && (sizeof(OT) == 4 || last)) {
                                 __syncwarp();
-                                const int n = p.cols - un.col0 - c_run;
-                                if (n > 0 && row_w < p.rows)
+                                const int col_w = un.col0 + half * HALF + c_run;
+                                if (col_w < p.cols && row_w < p.rows)
                                     store_runs<OT>(buf,
                                                    reinterpret_cast<OT *>(p.out) + un.split * p.out_split +
-                                                       (int64_t)row_w * p.out_pitch + un.col0 + c_run,
-                                                   p.out_pitch, p.rows - row_w, n, lane);
+                                                       (int64_t)row_w * p.out_pitch + col_w,
+                                                   p.out_pitch, p.rows - row_w, p.cols - col_w, lane);
                                 __syncwarp();
                             }
                         }
                     }
+                }
+            };
+            auto load = [&](uint32_t (&r)[STEP / 32][32], int c0) {
+#pragma unroll
+                for (int h = 0; h < STEP / 32; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
+            };
+            if (mine) {
+                uint32_t r0[STEP / 32][32], r1[STEP / 32][32];
+                const int c_first = STEPS == 2 && acc == 0 ? STEP : 0;
+                load(r0, c_first);
+                tmem_ld_wait();
+                if (STEPS == 2) load(r1, STEP - c_first);  // on its way while the first step is finished
+                if (shares && (S::OVERLAP || STEPS == 1)) release();
+                put(r0, c_first, STEPS == 1);
+                if constexpr (STEPS == 2) {
+                    tmem_ld_wait();
+                    if (shares && !S::OVERLAP) release();
+                    put(r1, STEP - c_first, true);
                 }
             }
             if (++acc == 2) {
@@ -675,7 +756,7 @@ template <typename OT, typename S, int STORE>
 int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tmOut, const GemmParams &p,
            cudaStream_t stream) {
     auto kern = block_gemm_kernel<OT, S, STORE>;
-    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + kEpilogueWarps * out_bytes<OT>(STORE) +
+    constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + kEpilogueWarps * out_bytes(STORE) +
                             kScaleSlots * S::SLOT_BYTES + sizeof(Shared);
     static_assert(smem <= 232448, "shared memory per block");
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -704,8 +785,8 @@ int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tm
 }
 
 // Operand stages: what the store buffers leave of shared memory.
-template <typename OT, int STORE>
-using Pair = Shape<true, kPairCols, STORE == kRows ? 4 : sizeof(OT) == 4 ? 5 : 6>;
+template <int STORE>
+using Pair = Shape<true, kPairCols, STORE == kRows ? 4 : 5>;
 using One32 = Shape<false, 32, 10>;
 using One64 = Shape<false, 64, 8>;
 using One128 = Shape<false, 128, 6>;
@@ -775,8 +856,8 @@ template <typename OT>
 int run_plan(const Plan &pl, int store, const CUtensorMap &r, const CUtensorMap &c, const CUtensorMap &o, const GemmParams &p,
              cudaStream_t s) {
     if (pl.pair)
-        return store == kTma ? launch<OT, Pair<OT, kTma>, kTma>(r, c, o, p, s)
-                             : launch<OT, Pair<OT, kRows>, kRows>(r, c, o, p, s);
+        return store == kTma ? launch<OT, Pair<kTma>, kTma>(r, c, o, p, s)
+                             : launch<OT, Pair<kRows>, kRows>(r, c, o, p, s);
     if (pl.cols == 32) return launch<OT, One32, kSwapped>(r, c, o, p, s);
     if (pl.cols == 64) return launch<OT, One64, kSwapped>(r, c, o, p, s);
     return launch<OT, One128, kSwapped>(r, c, o, p, s);

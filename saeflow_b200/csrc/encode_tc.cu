@@ -1386,11 +1386,10 @@ int make_map_out(CUtensorMap *map, const void *base, int dtype, uint64_t cols, u
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     cuuint64_t dims[3] = {cols, rows, splits};
     cuuint64_t strides[2] = {pitch_bytes, split_bytes};
-    cuuint32_t box[3] = {32, 32, 1};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / dtype_size(dtype)), 32, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(map, dt, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    dtype == SF_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                    CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return set_error(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for an output of %llu x %llu, pitch %llu",
                          (int)r, (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)pitch_bytes);

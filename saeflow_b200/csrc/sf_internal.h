@@ -138,8 +138,8 @@ int encode_tc_csr(const GemmOperands &g, const EpilogueArgs &ep, const CsrArgs &
 // swizzle, zeros past the extents (encode_tc.cu).
 int make_map_e4m3(CUtensorMap *map, const void *base, uint64_t cols, uint64_t rows, uint64_t pitch_bytes,
                   uint32_t box_rows);
-// Tensor map of `splits` row-major matrices of sf_dtype `dtype` for stores of 32 rows x 32 columns, swizzled
-// over their 128 (fp32) or 64 bytes (encode_tc.cu).
+// Tensor map of `splits` row-major matrices of sf_dtype `dtype` for stores of 32 rows x 128 bytes, 128-byte
+// swizzle (encode_tc.cu).
 int make_map_out(CUtensorMap *map, const void *base, int dtype, uint64_t cols, uint64_t rows, uint64_t splits,
                  uint64_t pitch_bytes, uint64_t split_bytes);
 int check_blocks(const sf_blocks *b, const char *name);
