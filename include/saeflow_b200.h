@@ -379,6 +379,26 @@ SF_API int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *
                            int activation, const sf_matrix *out, void *workspace, size_t workspace_bytes,
                            sf_stream stream);
 
+/*
+ * The 8-bit linear step y = Q(x) @ Q(W) + bias and its gradients, each a quantising pass per operand and
+ * products: x [M, K], W [K, N], every product's operands quantised along the axis that it sums over (W in
+ * tiles). `needs` is a set of bits: 1 dx, 2 dW, 4 the sums of dy. Of the forward, the backward reads only
+ * `keep` (Q(x^T) where dW is needed, Q(W) where dx is); temp is scratch of a call.
+ */
+SF_API int sf_linear8_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int W_dtype, int needs, size_t *keep,
+                            size_t *forward_temp, size_t *backward_temp);
+
+/* y [M, N] in x's dtype; bias fp32 [N] or NULL; needs: bits 1 and 2. */
+SF_API int sf_linear8_forward(const sf_matrix *x, const sf_matrix *W, const float *bias, const sf_matrix *y, int needs,
+                              void *keep, void *temp, size_t temp_bytes, sf_stream stream);
+
+/*
+ * From dy [M, N] (M > 0): dx [M, K] = Q(dy) @ Q(W)^T, dW [K, N] = Q(x^T) @ Q(dy^T)^T and db fp32 [N], the
+ * sums of dy over its rows; NULL where not wanted (`needs` is the forward's, which laid out `keep`).
+ */
+SF_API int sf_linear8_backward(const sf_matrix *dy, const void *keep, int64_t K, int needs, const sf_matrix *dx,
+                               const sf_matrix *dW, float *db, void *temp, size_t temp_bytes, sf_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,6 +90,10 @@ SIGNATURES = {
     "sf_blocks_quantize": (_c.c_int, [_MP, _BP, _BP, _P, _P, _c.c_size_t, _P]),
     "sf_block_matmul_workspace": (_c.c_int, [_BP, _BP, _MP, _SIZE_P]),
     "sf_block_matmul": (_c.c_int, [_BP, _BP, _P, _P, _c.c_int, _MP, _P, _c.c_size_t, _P]),
+    "sf_linear8_bytes": (_c.c_int, [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _SIZE_P, _SIZE_P,
+                                    _SIZE_P]),
+    "sf_linear8_forward": (_c.c_int, [_MP, _MP, _P, _MP, _c.c_int, _P, _P, _c.c_size_t, _P]),
+    "sf_linear8_backward": (_c.c_int, [_MP, _P, _c.c_int64, _c.c_int, _MP, _MP, _P, _P, _c.c_size_t, _P]),
     "sf_topk_encode_workspace": (_c.c_int, [_MP, _MP, _c.c_int, _c.c_int, _SIZE_P]),
     "sf_topk_encode": (_c.c_int, [_MP, _MP, _VP, _VP, _c.c_int, _P, _P, _c.c_int, _c.c_int, _P,
                                   _c.c_size_t, _P]),

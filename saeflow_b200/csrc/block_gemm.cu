@@ -638,23 +638,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             };
-            auto load = [&](uint32_t (&r)[STEP / 32][32], int c0) {
+            // One step's sums at a time: loading the second while the first is finished spilled registers, and
+            // was slower at every size measured (16384 x 256 x 65536: 773 against 638 us).
+            const int c_first = STEPS == 2 && acc == 0 ? STEP : 0;
+#pragma unroll 1
+            for (int i = 0; mine && i < STEPS; ++i) {
+                const int c0 = i == 0 ? c_first : STEP - c_first;
+                uint32_t r[STEP / 32][32];
 #pragma unroll
                 for (int h = 0; h < STEP / 32; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
-            };
-            if (mine) {
-                uint32_t r0[STEP / 32][32], r1[STEP / 32][32];
-                const int c_first = STEPS == 2 && acc == 0 ? STEP : 0;
-                load(r0, c_first);
                 tmem_ld_wait();
-                if (STEPS == 2) load(r1, STEP - c_first);  // on its way while the first step is finished
-                if (shares && (S::OVERLAP || STEPS == 1)) release();
-                put(r0, c_first, STEPS == 1);
-                if constexpr (STEPS == 2) {
-                    tmem_ld_wait();
-                    if (shares && !S::OVERLAP) release();
-                    put(r1, STEP - c_first, true);
-                }
+                if (shares && i == (S::OVERLAP ? 0 : STEPS - 1)) release();
+                put(r, c0, i == STEPS - 1);
             }
             if (++acc == 2) {
                 acc = 0;

@@ -28,14 +28,6 @@ def _cdiv(a, b):
     return -(-a // b)
 
 
-def _layout(rows, cols, tile):
-    """(data pitch, scale pitch, rows of scales, bytes of both from a 256-byte aligned start) of the smallest
-    aligned rows."""
-    dp, sp = _cdiv(cols, 16) * 16, _cdiv(cols, 4 * BLOCK) * 4
-    scale_rows = _cdiv(rows, BLOCK) if tile else rows
-    return dp, sp, scale_rows, _cdiv(rows * dp, 256) * 256 + _cdiv(scale_rows * sp, 256) * 256
-
-
 class BlockScaled:
     """An 8-bit matrix [rows, cols] on a CUDA device.
 
@@ -78,11 +70,11 @@ class BlockScaled:
         dev = torch.device("cuda" if device is None else device)
         if dev.type != "cuda":
             raise ValueError(f"device is {dev}; saeflow_b200 runs on CUDA devices only")
-        dp, sp, scale_rows, _ = _layout(rows, cols, tile)
+        nb = _cdiv(cols, BLOCK)
+        dp, sp, scale_rows = _cdiv(cols, 16) * 16, _cdiv(nb, 4) * 4, _cdiv(rows, BLOCK) if tile else rows
         data = torch.empty_strided((rows, cols), (dp, 1), dtype=_F8, device=dev)
         # a product reads scale bytes four at a time, so the padding is there; its values are never used
         scales = torch.empty(scale_rows, sp, dtype=torch.uint8, device=dev)
-        nb = _cdiv(cols, BLOCK)
         self = cls.__new__(cls)
         self.data, self.scales = data, scales if sp == nb else scales[:, :nb]
         self.tile, self.shape, self.device = bool(tile), (rows, cols), data.device
@@ -249,76 +241,37 @@ def _product(dev, a, b, bias, threshold, activation, out):
          ws.data_ptr() if need.value else None, need.value)
 
 
-class _Carver:
-    """Uninitialised BlockScaled structures in one buffer (a step needs up to four: one allocation, no views).
-    Add them, then place() the buffer; the structures are valid while it lives."""
-
-    __slots__ = ("parts", "bytes")
-
-    def __init__(self):
-        self.parts, self.bytes = [], 0
-
-    def add(self, rows, cols, tile):
-        dp, sp, scale_rows, size = _layout(rows, cols, tile)
-        c = _abi.SfBlocks(self.bytes, self.bytes + _cdiv(rows * dp, 256) * 256, rows, cols, dp, sp, int(tile), 0)
-        self.parts.append(c)
-        self.bytes += size
-        return c
-
-    def place(self, dev, buffer=None):
-        if buffer is None:
-            buffer = torch.empty(max(self.bytes, 1), dtype=torch.uint8, device=dev)
-        at = buffer.data_ptr()
-        for c in self.parts:
-            c.data = at + (c.data or 0)
-            c.scales = at + (c.scales or 0)
-        return buffer
-
-
-def linear8_forward(x, W, b, need_x, need_W):
-    """(y, buffer) of saeflow_b200.training.linear8: y = Q(x) @ Q(W) + b in x's dtype, and what its backward
-    reads: Q(x^T) where W needs a gradient, then Q(W) where x does (linear8_backward lays them out alike)."""
+def linear8_forward(x, W, b, needs):
+    """(y, kept, backward's scratch bytes) of saeflow_b200.training.linear8: y = Q(x) @ Q(W) + b in x's dtype, and the
+    buffer that its backward reads. needs: bits 1 dx, 2 dW, 4 db."""
     dev = _abi.require_cuda(("x", x), ("W", W), ("b", b))
     (M, K), N = x.shape, W.shape[1]
     xm, wm = _abi.matrix(x, "x"), _abi.matrix(W, "W")
     bias = _vector(b, "b", N, dev)
-    keep, temp = _Carver(), _Carver()
-    xt = keep.add(K, M, False) if need_W else None
-    wq = keep.add(K, N, True) if need_x else None
-    xq, wt = temp.add(M, K, False), temp.add(N, K, True)
-    kept, used = keep.place(dev) if need_W or need_x else None, temp.place(dev)
     lib = _abi.load()
-    _run(dev, lib.sf_blocks_quantize, ctypes.byref(xm), ctypes.byref(xq), _abi.ref(xt), None, None, 0)
-    _run(dev, lib.sf_blocks_quantize, ctypes.byref(wm), _abi.ref(wq), ctypes.byref(wt), None, None, 0)
+    keep, temp, later = ctypes.c_size_t(0), ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _abi.check(lib.sf_linear8_bytes(M, K, N, xm.dtype, wm.dtype, needs, ctypes.byref(keep), ctypes.byref(temp),
+                                    ctypes.byref(later)))
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
-    _product(dev, ctypes.byref(xq), ctypes.byref(wt), bias, None, -1, y)
-    del used  # stream-ordered: the allocator reuses it after these kernels
-    return y, kept
+    kept = torch.empty(keep.value, dtype=torch.uint8, device=dev) if keep.value else None
+    scratch = torch.empty(temp.value, dtype=torch.uint8, device=dev)
+    _run(dev, lib.sf_linear8_forward, ctypes.byref(xm), ctypes.byref(wm), bias.data_ptr() if bias is not None else None,
+         ctypes.byref(_abi.matrix(y, "y")), needs, kept.data_ptr() if keep.value else None, scratch.data_ptr(),
+         temp.value)
+    return y, kept, later.value
 
 
-def linear8_backward(dy, kept, M, K, N, x_dtype, W_dtype, need_x, need_W, need_b):
-    """(dx, dW, fp32 db) of linear8 from dy [M, N] and its forward's buffer; None where not needed. M > 0."""
+def linear8_backward(dy, kept, K, x_dtype, W_dtype, needs, scratch_bytes):
+    """(dx, dW, fp32 db) of linear8 from dy [M, N], M > 0, and its forward's buffer; None where not needed."""
     dev = _abi.require_cuda(("dy", dy))
     dm = _abi.matrix(dy, "dy")
-    keep, temp = _Carver(), _Carver()
-    xt = keep.add(K, M, False) if need_W else None
-    wq = keep.add(K, N, True) if need_x else None
-    if kept is not None:
-        keep.place(dev, kept)
-    dyq = temp.add(M, N, False) if need_x or not need_W else None
-    dyt = temp.add(N, M, False) if need_W else None
-    sums_at = temp.bytes
-    n = 4 * _cdiv(M, BLOCK) * N if need_b else 0
-    temp.bytes += n
-    used = temp.place(dev)
-    db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
-    _run(dev, _abi.load().sf_blocks_quantize, ctypes.byref(dm), _abi.ref(dyq), _abi.ref(dyt),
-         db.data_ptr() if need_b else None, used.data_ptr() + sums_at if need_b else None, n)
-    dx = dW = None
-    if need_x:
-        dx = torch.empty(M, K, dtype=x_dtype, device=dev)
-        _product(dev, ctypes.byref(dyq), ctypes.byref(wq), None, None, -1, dx)
-    if need_W:
-        dW = torch.empty(K, N, dtype=W_dtype, device=dev)
-        _product(dev, ctypes.byref(xt), ctypes.byref(dyt), None, None, -1, dW)
+    M, N = dy.shape
+    dx = torch.empty(M, K, dtype=x_dtype, device=dev) if needs & 1 else None
+    dW = torch.empty(K, N, dtype=W_dtype, device=dev) if needs & 2 else None
+    db = torch.empty(N, dtype=torch.float32, device=dev) if needs & 4 else None
+    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev)
+    _run(dev, _abi.load().sf_linear8_backward, ctypes.byref(dm), kept.data_ptr() if kept is not None else None, K, needs,
+         ctypes.byref(_abi.matrix(dx, "dx")) if needs & 1 else None,
+         ctypes.byref(_abi.matrix(dW, "dW")) if needs & 2 else None,
+         db.data_ptr() if needs & 4 else None, scratch.data_ptr(), scratch_bytes)
     return dx, dW, db

@@ -105,21 +105,23 @@ def forward(sae, x):
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b):
-        y, kept = linear8_forward(x, W, b, *ctx.needs_input_grad[:2])
+        need_x, need_W, need_b = ctx.needs_input_grad
+        needs = need_x + 2 * need_W + 4 * need_b
+        y, kept, scratch = linear8_forward(x, W, b, needs)
         ctx.save_for_backward(kept)
-        ctx.args = (*x.shape, W.shape[1], x.dtype, W.dtype)
+        ctx.args = x.shape[1], x.dtype, W.dtype, needs, scratch
         ctx.b_dtype = None if b is None else b.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        needs = ctx.needs_input_grad[:3]
-        M, K, N, x_dtype, W_dtype = ctx.args
+        K, x_dtype, W_dtype, needs, _ = ctx.args
+        M, N = dy.shape
         if not M:
-            return (dy.new_zeros(M, K, dtype=x_dtype) if needs[0] else None,
-                    dy.new_zeros(K, N, dtype=W_dtype) if needs[1] else None,
-                    dy.new_zeros(N, dtype=ctx.b_dtype) if needs[2] else None)
-        dx, dW, db = linear8_backward(dy, ctx.saved_tensors[0], *ctx.args, *needs)
+            return (dy.new_zeros(M, K, dtype=x_dtype) if needs & 1 else None,
+                    dy.new_zeros(K, N, dtype=W_dtype) if needs & 2 else None,
+                    dy.new_zeros(N, dtype=ctx.b_dtype) if needs & 4 else None)
+        dx, dW, db = linear8_backward(dy, ctx.saved_tensors[0], *ctx.args)
         return dx, dW, db if db is None or ctx.b_dtype == torch.float32 else db.to(ctx.b_dtype)
 
 
