@@ -96,16 +96,17 @@ class BlockScaled:
         return f"BlockScaled({list(self.shape)}, {'tiles' if self.tile else 'row blocks'}, {self.device})"
 
 
-def _run(dev, fn, *args):
-    """Call a library function on `dev`'s current stream."""
+def _run(dev, fn, *args, retry=None):
+    """Call a library function on `dev`'s current stream. True if it returned the status `retry`."""
     i = dev.index
     if torch._C._cuda_getDevice() == i:  # as torch.cuda.current_device, on an initialised device
         status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
             status = fn(*args, _abi.stream_of(dev))
-    if status:
+    if status and status != retry:
         _abi.check(status)
+    return status != 0
 
 
 def _index(t, name, n, dev):
@@ -230,15 +231,16 @@ def _vector(v, name, n, dev):
 
 
 def _product(dev, a, b, bias, threshold, activation, out):
-    """sf_block_matmul on ctypes references, with its workspace."""
+    """sf_block_matmul on ctypes references. Most products need no scratch: it is asked for when one does."""
     lib = _abi.load()
     m = ctypes.byref(_abi.matrix(out, "out"))
-    need = ctypes.c_size_t(0)
-    _abi.check(lib.sf_block_matmul_workspace(a, b, m, ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-    _run(dev, lib.sf_block_matmul, a, b, bias.data_ptr() if bias is not None else None,
-         threshold.data_ptr() if threshold is not None else None, activation, m,
-         ws.data_ptr() if need.value else None, need.value)
+    args = (a, b, bias.data_ptr() if bias is not None else None,
+            threshold.data_ptr() if threshold is not None else None, activation, m)
+    if _run(dev, lib.sf_block_matmul, *args, None, 0, retry=_abi.SF_ERR_WORKSPACE):
+        need = ctypes.c_size_t(0)
+        _abi.check(lib.sf_block_matmul_workspace(a, b, m, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        _run(dev, lib.sf_block_matmul, *args, ws.data_ptr(), need.value)
 
 
 def linear8_forward(x, W, b, needs):
