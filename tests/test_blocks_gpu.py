@@ -469,3 +469,17 @@ def test_refusals():
         store.view(3, 9)
     with pytest.raises(RuntimeError, match="unit column stride"):
         block_matmul(a, a, out=torch.empty(4, 4, device="cuda").T)
+
+
+def test_example_trains_and_encodes_from_the_store():
+    """examples/train_from_store.py at a small size: the loss falls, and the 8-bit encoder explains most of
+    the stored activations."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "train_from_store.py"
+    spec = importlib.util.spec_from_file_location("train_from_store", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    first, last, explained = example.main(["--rows", "8192", "--d-in", "192", "--d-sae", "1024", "--steps", "150"])
+    assert last < 0.6 * first and explained > 0.5
