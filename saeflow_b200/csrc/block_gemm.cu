@@ -44,7 +44,7 @@ struct GemmParams {
     int row_tiles, col_tiles;
     int col_bytes;             // the columns' operand per CTA and stage, as its TMA box is cut
     int group_rows;            // row tiles that run side by side over each column tile
-    Divisor by_tiles, by_group, by_rows, by_last_rows;  // tiles, tiles of a group, rows of a group, of the last
+    Divisor32 by_tiles, by_group, by_rows, by_last_rows;  // tiles, tiles of a group, rows of a group, of the last
     const uint8_t *r_scales, *c_scales;  // of the rows' and the columns' operand
     int64_t r_pitch, c_pitch;
     int r_shift, c_shift;      // log2 of the rows a scale row serves: 0 row blocks, 7 tiles
@@ -102,14 +102,14 @@ struct Unit {
 template <typename S>
 __device__ __forceinline__ Unit unit_of(const GemmParams &p, int u) {
     Unit r;
-    r.split = (int)p.by_tiles.div(u);
+    r.split = p.by_tiles.div(u);
     u -= r.split * (int)p.by_tiles.d;
-    const int g = (int)p.by_group.div(u);
+    const int g = p.by_group.div(u);
     const int first = g * p.group_rows;
     const bool last = p.row_tiles - first < p.group_rows;
-    const Divisor by = last ? p.by_last_rows : p.by_rows;
+    const Divisor32 by = last ? p.by_last_rows : p.by_rows;
     const int local = u - g * (int)p.by_group.d;
-    const int col = (int)by.div(local);
+    const int col = by.div(local);
     r.row0 = (first + local - col * (int)by.d) * S::ROWS;
     r.col0 = col * S::COLS;
     r.kb0 = 4 * r.split * p.split_groups;
@@ -367,6 +367,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         else
             mbar_arrive(bar);
     };
+    // For TMEM that has been read.
+    auto release_leader = [&](uint64_t *bar) {
+        if (PAIR)
+            mbar_arrive_remote_cta(map_to_rank(smem_u32(bar), 0));
+        else
+            mbar_arrive(bar);
+    };
     // Completion of the MMA thread's work so far, on this barrier of every CTA.
     auto commit = [&](uint64_t *bar) {
         if (PAIR) {
@@ -527,8 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int OWN = SWAP ? 1 : HALF / 32;
         float next_bias[OWN], next_thr[OWN];
         float *my_bias = sh->bias[warp - 2], *my_thr = sh->thr[warp - 2];
-        auto load_vectors = [&](int u) {
-            const Unit un = unit_of<S>(p, min(u, units - 1));
+        auto load_vectors = [&](const Unit &un) {
 #pragma unroll
             for (int j = 0; j < OWN; ++j) {
                 const int at = SWAP ? un.row0 + (int)rank * kRowTile + quad * 32 + lane
@@ -538,9 +544,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 next_thr[j] = p.thr && have ? __ldg(p.thr + at) : 0.f;
             }
         };
-        load_vectors(first_unit);
+        Unit next = unit_of<S>(p, min(first_unit, units - 1));
+        load_vectors(next);
         for (int u = first_unit; u < units; u += step_units) {
-            const Unit un = unit_of<S>(p, u);
+            const Unit un = next;
             const int row = un.row0 + (int)rank * kRowTile + quad * 32 + lane;
             const float row_bias = next_bias[0], row_thr = next_thr[0];
             if (!SWAP) {
@@ -551,7 +558,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
             }
-            load_vectors(u + step_units);
+            next = unit_of<S>(p, min(u + step_units, units - 1));
+            load_vectors(next);
             if (!wait(&sh->tmem_full[acc], acc_phase)) break;
             tc_fence_after();
             const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1 + half * HALF;
@@ -562,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto release = [&]() {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_leader(&sh->tmem_empty[acc]);
+                if (lane == 0) release_leader(&sh->tmem_empty[acc]);
             };
             if (!shares || !mine) release();
 
@@ -915,10 +923,10 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     // A group of row tiles runs side by side over each column tile: the columns' operand is read from HBM
     // once per group, while the group's 32 MB stay in L2.
     p.group_rows = (int)std::max<int64_t>(1, std::min<int64_t>(p.row_tiles, (int64_t(32) << 20) / (row_tile * a->cols)));
-    p.by_tiles = Divisor::of(p.row_tiles * p.col_tiles);
-    p.by_group = Divisor::of(p.group_rows * p.col_tiles);
-    p.by_rows = Divisor::of(p.group_rows);
-    p.by_last_rows = Divisor::of(p.row_tiles % p.group_rows ? p.row_tiles % p.group_rows : p.group_rows);
+    p.by_tiles = Divisor32::of(p.row_tiles * p.col_tiles);
+    p.by_group = Divisor32::of(p.group_rows * p.col_tiles);
+    p.by_rows = Divisor32::of(p.group_rows);
+    p.by_last_rows = Divisor32::of(p.row_tiles % p.group_rows ? p.row_tiles % p.group_rows : p.group_rows);
     p.r_scales = static_cast<const uint8_t *>(R->scales);
     p.c_scales = static_cast<const uint8_t *>(C->scales);
     p.r_pitch = R->scale_pitch;

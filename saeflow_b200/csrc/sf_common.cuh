@@ -73,6 +73,23 @@ struct Divisor {
     }
 };
 
+// Division of 0 <= n < 2^32 in five instructions (Granlund and Montgomery, Division by invariant integers using
+// multiplication, 1994, figure 4.1).
+struct Divisor32 {
+    uint32_t magic, d;
+    int s1, s2;
+    __host__ static Divisor32 of(uint32_t d) {
+        int l = 0;
+        while ((1ull << l) < d) ++l;
+        const uint32_t m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+        return Divisor32{m, d, l < 1 ? l : 1, l > 1 ? l - 1 : 0};
+    }
+    __device__ __forceinline__ int div(int n) const {
+        const uint32_t t = __umulhi(magic, (uint32_t)n);
+        return (int)((t + (((uint32_t)n - t) >> s1)) >> s2);
+    }
+};
+
 // ---------------------------------------------------------------------------------------
 // Shared-memory addressing, timers
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -372,6 +389,11 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t ran
 }
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same without ordering memory across the cluster, for a phase that passes on no written memory (TMEM that
+// has been read): the release at cluster scope waits for the thread's stores, some 700 clocks behind an epilogue.
+__device__ __forceinline__ void mbar_arrive_remote_cta(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void st_remote_u32(uint32_t cluster_addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
