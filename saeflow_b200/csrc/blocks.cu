@@ -117,37 +117,31 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Words of the 16 elements from column k of a row, zeros past K. `base` is the row's first element. Rows
-// with a unit column stride are read in aligned 16-byte pieces and shifted into place, so any alignment
-// of the element type costs one more piece and a few selects.
+// The 16 elements from column k of a row, zeros past K, in two steps so that several rows' loads can be under
+// way before the first is used. `base` is the row's first element. Rows with a unit column stride are read in
+// aligned 16-byte pieces and shifted into place, so any alignment of the element type costs one more piece
+// and a few selects.
 template <typename XT>
-__device__ __forceinline__ void load16(const XT *base, int64_t k, int64_t K, int64_t sxk, uint32_t *v) {
+struct Fetched {
+    uint32_t w[Held<XT>::WORDS + 4];
+    unsigned off;  // bytes of the first piece before the first element
+};
+
+template <typename XT>
+__device__ __forceinline__ void fetch16(const XT *base, int64_t k, int64_t K, int64_t sxk, Fetched<XT> &f) {
     using H = Held<XT>;
     constexpr int W = H::WORDS, PER = 16 / W;
+    f.off = 0;
     if (sxk == 1 && k + 16 <= K) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(base + k);
         const uint4 *p = reinterpret_cast<const uint4 *>(at & ~uintptr_t(15));
-        const unsigned off = (unsigned)at & 15u;
-        if (off == 0) {
-#pragma unroll
-            for (int j = 0; j < W; j += 4) {
-                const uint4 a = __ldg(p + j / 4);
-                v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
-            }
-            return;
-        }
-        uint32_t w[W + 4];  // the last piece holds the last element, as off > 0
+        f.off = (unsigned)at & 15u;
 #pragma unroll
         for (int j = 0; j < W + 4; j += 4) {
+            if (j == W && f.off == 0) break;  // with off > 0 the last piece holds the last element
             const uint4 a = __ldg(p + j / 4);
-            w[j] = a.x, w[j + 1] = a.y, w[j + 2] = a.z, w[j + 3] = a.w;
+            f.w[j] = a.x, f.w[j + 1] = a.y, f.w[j + 2] = a.z, f.w[j + 3] = a.w;
         }
-#pragma unroll
-        for (int j = 0; j < W + 2; ++j) w[j] = (off & 8) ? w[j + 2] : w[j];
-#pragma unroll
-        for (int j = 0; j < W + 1; ++j) w[j] = (off & 4) ? w[j + 1] : w[j];
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = H::HALF && (off & 2) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
         return;
     }
 #pragma unroll
@@ -157,10 +151,38 @@ __device__ __forceinline__ void load16(const XT *base, int64_t k, int64_t K, int
         for (int i = 0; i < PER; ++i)
             e[i] = k + j * PER + i < K ? __ldg(base + (k + j * PER + i) * sxk) : from_f32<XT>(0.f);
         if constexpr (PER == 1)
-            v[j] = __float_as_uint(to_f32(e[0]));
+            f.w[j] = __float_as_uint(to_f32(e[0]));
         else
-            v[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(&e[0]) |
-                   (uint32_t)*reinterpret_cast<const uint16_t *>(&e[1]) << 16;
+            f.w[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(&e[0]) |
+                     (uint32_t)*reinterpret_cast<const uint16_t *>(&e[1]) << 16;
+    }
+}
+
+template <typename XT>
+__device__ __forceinline__ void place16(Fetched<XT> &f, uint32_t *v) {
+    using H = Held<XT>;
+    constexpr int W = H::WORDS;
+    if (f.off) {
+#pragma unroll
+        for (int j = 0; j < W + 2; ++j) f.w[j] = (f.off & 8) ? f.w[j + 2] : f.w[j];
+#pragma unroll
+        for (int j = 0; j < W + 1; ++j) f.w[j] = (f.off & 4) ? f.w[j + 1] : f.w[j];
+        if (H::HALF && (f.off & 2)) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) f.w[j] = __funnelshift_r(f.w[j], f.w[j + 1], 16);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = f.w[j];
+}
+
+// Aligned and inside the matrix: the words as they lie.
+template <typename XT>
+__device__ __forceinline__ void load16_aligned(const XT *src, uint32_t *v) {
+#pragma unroll
+    for (int j = 0; j < Held<XT>::WORDS; j += 4) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(src) + j / 4);
+        v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
     }
 }
 
@@ -180,7 +202,7 @@ __device__ __forceinline__ uint4 pack16(const uint32_t *v, float inv) {
 // (`by` divides by the pairs of a row), so that enough bytes are on their way.
 template <typename XT>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const XT *__restrict__ x, int64_t n, int64_t K, int64_t sxm,
-                                                         int64_t sxk, const int64_t *__restrict__ slots,
+                                                         int64_t sxk, bool vec, const int64_t *__restrict__ slots,
                                                          uint8_t *__restrict__ q, int64_t q_pitch,
                                                          uint8_t *__restrict__ s, int64_t s_pitch, int64_t cap,
                                                          Divisor by, unsigned *err) {
@@ -200,20 +222,27 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const XT *__restrict__ 
     // Sixteen columns from 16l; of aligned fp32 rows four from 4l of each 32, so that the group's 16-byte loads
     // are side by side.
     const XT *src = x + row * sxm;
-    const bool quads = !H::HALF && sxk == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0 && (2 * pair + 2) * kBlk <= K;
     uint32_t v[2][H::WORDS];
+    const bool whole = vec && (2 * pair + 2) * kBlk <= K;
+    const bool quads = !H::HALF && whole;
+    if (quads) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const int64_t k = (2 * pair + b) * kBlk;
-        if (!H::HALF && quads) {
+        for (int b = 0; b < 2; ++b) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint4 a = __ldg(reinterpret_cast<const uint4 *>(src + k) + 8 * j + l);
+            for (int j = 0; j < H::WORDS / 4; ++j) {
+                const uint4 a = __ldg(reinterpret_cast<const uint4 *>(src + (2 * pair + b) * kBlk) + 8 * j + l);
                 v[b][4 * j] = a.x, v[b][4 * j + 1] = a.y, v[b][4 * j + 2] = a.z, v[b][4 * j + 3] = a.w;
             }
-        } else {
-            load16(src, k + 16 * l, K, sxk, v[b]);
         }
+    } else if (whole) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) load16_aligned(src + (2 * pair + b) * kBlk + 16 * l, v[b]);
+    } else {
+        Fetched<XT> f[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) fetch16(src, (2 * pair + b) * kBlk + 16 * l, K, sxk, f[b]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) place16(f[b], v[b]);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -370,7 +399,7 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint8_t *__restric
 // pairs for the maxima; only a tile that holds an infinity or NaN looks at each of them.
 template <typename XT, bool TILE>
 __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
-    quant_tile_kernel(const XT *__restrict__ x, int64_t R, int64_t C, int64_t sxm, int64_t sxk, uint8_t *__restrict__ q,
+    quant_tile_kernel(const XT *__restrict__ x, int64_t R, int64_t C, int64_t sxm, int64_t sxk, bool vec, uint8_t *__restrict__ q,
                       int64_t q_pitch, uint8_t *__restrict__ qs, int64_t qs_pitch,
                       uint8_t *__restrict__ t, int64_t t_pitch, uint8_t *__restrict__ ts, int64_t ts_pitch,
                       float *__restrict__ sums) {
@@ -387,8 +416,19 @@ __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
     const int64_t r0 = rb * kBlk + rl, c0 = cb * kBlk + 16 * l;
 
     uint32_t v[4][W];
+    if (vec && r0 + 4 <= R && c0 + 16 <= C) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load16(x + (r0 + i) * sxm, c0, r0 + i < R ? C : 0, sxk, v[i]);
+        for (int i = 0; i < 4; ++i) load16_aligned(x + (r0 + i) * sxm + c0, v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            Fetched<XT> f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) fetch16(x + (r0 + i + h) * sxm, c0, r0 + i + h < R ? C : 0, sxk, f[h]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) place16(f[h], v[i + h]);
+        }
+    }
     if (sums) {  // each thread's four rows; quad j of lane l at quad 4l + (j + l / 2) % 4, without bank conflicts
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
@@ -602,8 +642,8 @@ int sf_blocks_write(const sf_matrix *x, const int64_t *slots, const sf_blocks *d
     return with_type(x->dtype, [&](auto tag) {
         using T = decltype(tag);
         quant_rows_kernel<T><<<grid, 256, 0, s>>>(
-            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col, slots,
-            static_cast<uint8_t *>(dst->data), dst->data_pitch, static_cast<uint8_t *>(dst->scales), dst->scale_pitch,
+            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col, vector_rows(*x),
+            slots, static_cast<uint8_t *>(dst->data), dst->data_pitch, static_cast<uint8_t *>(dst->scales), dst->scale_pitch,
             dst->rows, by, device_error_word());
         return check_cuda(cudaGetLastError(), "quant_rows launch");
     });
@@ -694,7 +734,7 @@ int sf_blocks_quantize(const sf_matrix *x, const sf_blocks *q, const sf_blocks *
         using T = decltype(tag);
         auto kern = tile ? quant_tile_kernel<T, true> : quant_tile_kernel<T, false>;
         kern<<<dim3((unsigned)ncb, (unsigned)nrb), 256, 0, s>>>(
-            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col,
+            reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col, vector_rows(*x),
             static_cast<uint8_t *>(a.data), a.data_pitch, static_cast<uint8_t *>(a.scales), a.scale_pitch,
             static_cast<uint8_t *>(b.data), b.data_pitch, static_cast<uint8_t *>(b.scales), b.scale_pitch, part);
         return check_cuda(cudaGetLastError(), "quant_tile launch");
