@@ -19,6 +19,16 @@
 // operand; both CTAs' loads complete on the leader's barriers. Single: one CTA computes 128 x COLS.
 // A pair's tile has rows of `a` for its rows (TMEM lanes); a single CTA's has rows of `b`, so that few rows of
 // `a` make a narrow tile (COLS = 32) beside 128 rows of weights.
+//
+// What bounds it. A pair reads 64 KB of operands from L2 per K block; all 148 SMs together get about 6 KB a
+// clock, 700 to 780 clocks a block, where the MMAs take 512 (530 measured with the loads left out): large
+// products are bound by operand delivery, and in a steady loop by the 1000 W power cap (SM clock near
+// 1.4 GHz). Few rows of `a` are bound by the bytes of `b`, K below some 1500 by the epilogue (about 3300
+// clocks a tile). Two accumulators of 256 columns and the scales exceed TMEM, so the accumulators overlap;
+// 224-column tiles, whose accumulators do not, move 7% more bytes and were slower at every K from 128 up.
+// Measured on a B200, bf16 outputs (M x K x N): 16384 x 2304 x 65536 1.95 ms, 2.5 PFLOP/s (in a steady loop 2.3 ms,
+// 2.15 PFLOP/s, 0.92 of the library's 8-bit product with one scale per tensor); 4096 x 768 x 16384 66 us;
+// 1 x 2304 x 65536 30.5 us, 5.0 TB/s of weights.
 #include <algorithm>
 #include <type_traits>
 
@@ -31,7 +41,7 @@ namespace {
 
 constexpr int kKBytes = 128;                   // elements (bytes) of K per stage
 constexpr int kScaleSlots = 3;                 // scale words of 512 elements of K each
-constexpr int kEpilogueWarps = 8;               // two for each quarter of the TMEM lanes
+constexpr int kEpilogueWarps = 8;              // two for each quarter of the TMEM lanes
 constexpr int kThreads = 32 * (3 + kEpilogueWarps);
 constexpr int kTmemCols = 512;
 constexpr int kPairCols = 256;                 // columns of a pair's tile
@@ -807,8 +817,10 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int out_dtype) {
     Plan pl{};
     const int sms = num_sms();
     const int groups = cdiv(K, 4 * kKBytes);
-    // Either kernel is paced by its operand loads, 128 + columns rows per K block and
-    // CTA (a pair's CTA loads half of its columns), and a pair's tile is twice the work per CTA.
+    // Either kernel is paced by its operand loads: 128 + cols rows per K block for a single CTA, 256 for a CTA of
+    // a pair, whose tile is twice the work. Waves times that predict the faster one; measured (us, pair against
+    // single): 256 x 768 x 16384 11.8 / 16.8, 512 x 512 x 5000 8.7 / 13.7, 2048 x 1024 x 2048 11.3 / 16.0, and
+    // about even where both fit one wave (200 x 768 x 5000: 9.6 / 9.7).
     const int cols = M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const int64_t one_tiles = (int64_t)cdiv(N, 128) * cdiv(M, cols);
     const int64_t pair_tiles = (int64_t)cdiv(N, 256) * cdiv(M, 256);
@@ -817,8 +829,10 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int out_dtype) {
     pl.cols = pl.pair ? kPairCols : cols;
     const int64_t tiles = pl.pair ? pair_tiles : one_tiles;
     const int slots = pl.pair ? sms / 2 : sms;
-    // Few tiles: K is split among the idle SMs, 512 elements at least to each, and the partial sums joined.
-    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(groups, slots / tiles));
+    // Few tiles: K is split among the idle SMs, at least 2048 of it to each, and the partial sums joined by a
+    // second kernel. Measured (us, split against whole): K = 768 12.7 / 9.5 (512 x 2048), 2304 13.0 / 12.4
+    // (256 x 2048), 5000 19.3 / 23.6 (1000 x 768), 8192 16.1 / 24.4 (640 x 640), 13558 23.5 / 35.1 (636 x 1094).
+    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(groups / 4, slots / tiles));
     // The tensor cores round each addition toward zero, a bias that grows with the number of additions
     // (measured against 64 bits: 9e-7 of the result at K = 8192, 1.2e-5 at 65536), far below a 16-bit
     // output's rounding but not an fp32 one's: those sum ranges of at most 8192, joined in fp32.
