@@ -114,6 +114,7 @@ class _Linear8(torch.autograd.Function):
         return y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         K, x_dtype, W_dtype, needs, _ = ctx.args
         M, N = dy.shape
@@ -135,9 +136,11 @@ def linear8(x, W, b=None):
     computes (y and dx: x's, dW: W's):
         y  = Q(x) @ Q(W) + b        dx = Q(dy) @ Q(W)^T
         dW = Q(x^T) @ Q(dy^T)^T     db = sum_rows dy   (dy as it is, fp32, in a fixed order)
-    The quantisation itself is taken as the identity (straight through)."""
+    The quantisation itself is taken as the identity (straight through); once differentiable."""
     if x.dim() != 2 or W.dim() != 2 or x.shape[1] != W.shape[0]:
         raise ValueError(f"linear8 takes x [M, K] and W [K, N], got {tuple(x.shape)} and {tuple(W.shape)}")
     if b is not None and tuple(b.shape) != (W.shape[1],):
         raise ValueError(f"b must be [{W.shape[1]}], got {tuple(b.shape)}")
+    if not torch.is_grad_enabled():  # only the product: nothing is laid out for a backward
+        return linear8_forward(x, W, b, 0)[0]
     return _Linear8.apply(x, W, b)

@@ -383,6 +383,57 @@ def test_linear8_needs_only_what_is_asked():
     close(dW, want[2], mags[2], 40, torch.float32)
 
 
+def test_linear8_without_gradients_and_twice():
+    x, W, b = (torch.randn(*s, device="cuda").requires_grad_() for s in ((30, 64), (64, 40), (40,)))
+    y = linear8(x, W, b)
+    with torch.no_grad():
+        assert torch.equal(linear8(x, W, b), y) and not linear8(x, W, b).requires_grad
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+def test_linear8_on_another_stream():
+    """Forward and backward on a side stream, behind a slow kernel there."""
+    x, W, b, dy = torch.randn(200, 96), torch.randn(96, 150), torch.randn(150), torch.randn(200, 150)
+    g = [t.cuda().requires_grad_() for t in (x, W, b)]
+    gdy = dy.cuda()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got = torch.autograd.grad(linear8(*g), g, gdy)
+    side.synchronize()
+    want = torch.autograd.grad(linear8(*g), g, gdy)
+    for a, w in zip(got, want):
+        assert torch.equal(a, w)
+
+
+def test_operators_in_a_graph():
+    """Captured once, replayed on new values in the same memory."""
+    x, W = torch.randn(300, 200, device="cuda"), torch.randn(500, 200, device="cuda")
+    store = ActivationStore(400, 200)
+    slots = torch.arange(300, device="cuda")
+    w8 = quantize(W, tile=True)
+
+    def step():
+        store.write(x, slots)
+        return block_matmul(store.view(0, 300), w8), store.read(slots, torch.float32), quantize_both(x, col_sums=True)[2]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step()
+    for _ in range(2):
+        x.normal_()
+        graph.replay()
+        for got, want in zip(out, step()):
+            assert torch.equal(got, want)
+
+
 def test_linear8_without_rows():
     x, W, b = (torch.randn(*s, device="cuda").requires_grad_() for s in ((0, 64), (64, 32), (32,)))
     y = linear8(x, W, b)
