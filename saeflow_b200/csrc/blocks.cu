@@ -39,14 +39,11 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, float *v) {
     }
 }
 
-// Eight e4m3 bytes from column k of a row of K columns; nothing past them is read.
-__device__ __forceinline__ uint2 load8_e4m3(const uint8_t *row, int64_t k, int64_t K) {
-    if (k + 8 <= K) return __ldg(reinterpret_cast<const uint2 *>(row + k));
-    uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (k + j < K) w[j >> 2] |= (uint32_t)__ldg(row + k + j) << (8 * (j & 3));
-    return make_uint2(w[0], w[1]);
+// The aligned word of a row's e4m3 bytes at column k, a multiple of 4; 0 outside the K columns. A word that
+// holds a column may also hold bytes past the last, which no one uses.
+template <typename I>
+__device__ __forceinline__ uint32_t load_word(const uint8_t *row, I k, I K) {
+    return k >= 0 && k < K ? __ldg(reinterpret_cast<const uint32_t *>(row + k)) : 0u;
 }
 
 // Eight e4m3 bytes at column k of a row of `limit` columns; nothing past them is written.
@@ -304,16 +301,16 @@ __device__ __forceinline__ void store_pair(__half *o, float a, float b) {
 // Bound by HBM: 16384 of 262144 rows of 2304 as bf16 in 17.9 us, 6.3 TB/s; as fp32 (four bytes written for one
 // read) 65536 rows in 140 us, 5.4 TB/s. Rows that start between boundaries: 5000 x 1001 fp16 10.5 us.
 template <typename OT, bool ALIGNED>
-__global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t *__restrict__ q, int64_t q_pitch,
+__global__ void __launch_bounds__(256, 4) read_rows_kernel(const uint8_t *__restrict__ q, int64_t q_pitch,
                                                         const uint8_t *__restrict__ s, int64_t s_pitch,
-                                                        int64_t src_rows, int64_t K, int tile_shift,
+                                                        int64_t src_rows, int K, int tile_shift,
                                                         const int64_t *__restrict__ rows, OT *__restrict__ out,
                                                         int64_t n, int64_t out_pitch, Divisor by, unsigned *err) {
     constexpr int PIECES = kReadElements<OT> / 8;
     const int64_t group = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
     const int64_t i = by.div(group);
     if (i >= n) return;
-    const int64_t c = (group - i * by.d) * 8 * PIECES + (threadIdx.x & 7);
+    const int c = (int)(group - i * by.d) * 8 * PIECES + (threadIdx.x & 7);
     int64_t row = i;
     if (rows) {
         row = __ldg(rows + i);
@@ -327,40 +324,32 @@ __global__ void __launch_bounds__(256) read_rows_kernel(const uint8_t *__restric
     uint32_t sb[PIECES][2];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int64_t k = (c + 8 * p) * 8 - shift;  // may start before the row, or end past it
+        const int k = (c + 8 * p) * 8 - shift;  // may start before the row, or end past it
         w[p] = make_uint2(0u, 0u);
         sb[p][0] = sb[p][1] = 0;
         if (!have || k >= K || k + 8 <= 0) continue;
-        sb[p][0] = __ldg(sc + max(k, (int64_t)0) / kBlk);
-        if (!ALIGNED) sb[p][1] = __ldg(sc + (min(k + 8, K) - 1) / kBlk);
+        sb[p][0] = __ldg(sc + (max(k, 0) >> 7));
+        if (!ALIGNED) sb[p][1] = __ldg(sc + ((min(k + 8, K) - 1) >> 7));
         if (ALIGNED && k + 8 <= K) {
             w[p] = __ldg(reinterpret_cast<const uint2 *>(src + k));
-        } else if (!ALIGNED && (k & ~int64_t(3)) >= 0 && (k & ~int64_t(3)) + 12 <= K) {
-            const uint32_t *a = reinterpret_cast<const uint32_t *>(src + (k & ~int64_t(3)));
-            const uint32_t a0 = __ldg(a), a1 = __ldg(a + 1), a2 = __ldg(a + 2);
-            const int bits = 8 * (int)(k & 3);
-            w[p] = make_uint2(__funnelshift_r(a0, a1, bits), __funnelshift_r(a1, a2, bits));
+        } else if (ALIGNED) {
+            w[p] = make_uint2(load_word(src, k, K), load_word(src, k + 4, K));
         } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k + j >= 0 && k + j < K) {
-                    const uint32_t byte = (uint32_t)__ldg(src + k + j) << (8 * (j & 3));
-                    if (j < 4)
-                        w[p].x |= byte;
-                    else
-                        w[p].y |= byte;
-                }
+            const int k4 = k & ~3;
+            const uint32_t a0 = load_word(src, k4, K), a1 = load_word(src, k4 + 4, K), a2 = load_word(src, k4 + 8, K);
+            const int bits = 8 * (k & 3);
+            w[p] = make_uint2(__funnelshift_r(a0, a1, bits), __funnelshift_r(a1, a2, bits));
         }
     }
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-        const int64_t k = (c + 8 * p) * 8 - shift;
+        const int k = (c + 8 * p) * 8 - shift;
         if (k >= K) break;
         float v[8];
         unpack_e4m3(w[p].x, v);
         unpack_e4m3(w[p].y, v + 4);
         const float s0 = have ? scale_value(sb[p][0]) : 0.f, s1 = ALIGNED ? s0 : have ? scale_value(sb[p][1]) : 0.f;
-        const int64_t turn = (k + 7) / kBlk * kBlk;  // columns from here have the second scale
+        const int turn = (k + 7) & ~(kBlk - 1);  // columns from here have the second scale
         alignas(16) OT o[8];
 #pragma unroll
         for (int j = 0; j < 8; j += 2)
@@ -391,7 +380,8 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const uint8_t *__restric
     if (row >= src_rows && lane == 0) atomicOr(err, kErrIndex);
     const bool have = row >= 0 && row < src_rows;
     for (int64_t k = 8 * lane; k < K; k += 256) {
-        const uint2 w = have ? load8_e4m3(q + row * q_pitch, k, K) : make_uint2(0u, 0u);
+        const uint8_t *src = q + row * q_pitch;
+        const uint2 w = have ? make_uint2(load_word(src, k, K), load_word(src, k + 4, K)) : make_uint2(0u, 0u);
         store8(oq + i * oq_pitch, k, K, w);
     }
     for (unsigned b = lane; b < nb; b += 32) os[i * os_pitch + b] = have ? __ldg(s + row * s_pitch + b) : (uint8_t)0;
@@ -665,6 +655,7 @@ int sf_blocks_read(const sf_blocks *src, const int64_t *rows, const sf_matrix *o
     if (!rows && out->rows > src->rows) return set_error(SF_ERR_INVALID, "out has more rows than src");
     if (out->rows == 0 || out->cols == 0) return SF_OK;
     if (out->stride_col != 1) return set_error(SF_ERR_UNSUPPORTED, "out needs a unit column stride");
+    if (out->cols > INT32_MAX - 4096) return set_error(SF_ERR_UNSUPPORTED, "too many columns");
     const bool aligned = vector_rows(*out);
     // a row's pieces of eight, one more where rows start between boundaries
     const int64_t pieces = (out->cols + 7) / 8 + (aligned ? 0 : 1);
@@ -678,7 +669,7 @@ int sf_blocks_read(const sf_blocks *src, const int64_t *rows, const sf_matrix *o
         auto kern = aligned ? read_rows_kernel<T, true> : read_rows_kernel<T, false>;
         kern<<<grid, 256, 0, s>>>(
             static_cast<const uint8_t *>(src->data), src->data_pitch, static_cast<const uint8_t *>(src->scales),
-            src->scale_pitch, src->rows, src->cols, src->tile ? 7 : 0, rows,
+            src->scale_pitch, src->rows, (int)src->cols, src->tile ? 7 : 0, rows,
             reinterpret_cast<T *>(const_cast<void *>(out->data)), out->rows, out->stride_row, by, device_error_word());
         return check_cuda(cudaGetLastError(), "read_rows launch");
     });
