@@ -371,6 +371,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         st_remote_u32(peer_abort, 1u);
         return false;
     };
+    // A whole warp waits: every lane sees the phase, and all of them agree on whether it came, so that a wait that
+    // ran out does not split the warp before an instruction that needs all of it (at most 1% of the time; one
+    // polling lane that the others follow cost 5 to 25%).
+    auto wait_warp = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+    auto wait_warp_cluster = [&](uint64_t *bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait_cluster(bar, parity)) != 0;
+    };
     auto arrive_leader = [&](uint64_t *bar) {
         if (PAIR)
             mbar_arrive_remote(map_to_rank(smem_u32(bar), 0));
@@ -456,15 +463,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // Accumulators that overlap: the previous tile's epilogue must have read the columns that
                 // this tile's shares with it (and so has finished the tile before that).
                 if (S::OVERLAP) {
-                    if (!first_tile && !(ok = wait(&sh->tmem_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1u))) break;
+                    if (!first_tile && !(ok = wait_warp(&sh->tmem_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1u))) break;
                     first_tile = false;
-                } else if (!(ok = wait(&sh->tmem_empty[acc], acc_phase ^ 1u))) {
+                } else if (!(ok = wait_warp(&sh->tmem_empty[acc], acc_phase ^ 1u))) {
                     break;
                 }
                 tc_fence_after();
                 const uint32_t d = tmem_u + acc * S::ACC1;
                 for (int kb4 = un.kb0; ok && kb4 < un.kb1; kb4 += 4) {
-                    if (!(ok = wait_cluster(&sh->scale_full[slot], slot_phase))) break;
+                    if (!(ok = wait_warp_cluster(&sh->scale_full[slot], slot_phase))) break;
                     tc_fence_after();
                     const uint32_t scales = tmem_u + S::SCALE_COL + slot * S::SLOT_COLS;
                     if (elect_one()) {
@@ -481,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         if (kb4 + j >= un.kb1) break;
-                        if (!(ok = wait(&sh->full[stage], phase))) break;
+                        if (!(ok = wait_warp(&sh->full[stage], phase))) break;
                         tc_fence_after();
                         const uint64_t rd = desc_r + stage * (S::R_BYTES >> 4), cd = desc_c + stage * (S::C_BYTES >> 4);
                         constexpr uint32_t IDESC0 = make_idesc_e4m3_scaled(S::ROWS, S::COLS, 0);
@@ -570,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             next = unit_of<S>(p, min(u + step_units, units - 1));
             load_vectors(next);
-            if (!wait(&sh->tmem_full[acc], acc_phase)) break;
+            if (!wait_warp(&sh->tmem_full[acc], acc_phase)) break;
             tc_fence_after();
             const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1 + half * HALF;
             // Overlapping accumulators: the shared columns (the first's last 40, the second's first 40) are
@@ -705,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (u < units) load();
-            if (!wait(&sh->scale_empty[slot], phase ^ 1u)) break;
+            if (!wait_warp(&sh->scale_empty[slot], phase ^ 1u)) break;
             uint8_t *dst = sScale + slot * S::SLOT_BYTES + lane * 16;
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) *reinterpret_cast<uint4 *>(dst + 512 * i) = now[i];

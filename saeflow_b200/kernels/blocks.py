@@ -14,6 +14,7 @@ The reference has neither (it keeps activations in 16 or 32 bits).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -243,6 +244,16 @@ def _product(dev, a, b, bias, threshold, activation, out):
         _run(dev, lib.sf_block_matmul, *args, ws.data_ptr(), need.value)
 
 
+@functools.lru_cache(maxsize=256)
+def _linear8_bytes(M, K, N, x_code, W_code, needs, device_index):
+    """Sizes of a step's buffers: they depend on the extents alone (and on the device's SM count)."""
+    keep, temp, later = ctypes.c_size_t(0), ctypes.c_size_t(0), ctypes.c_size_t(0)
+    with torch.cuda.device(device_index):
+        _abi.check(_abi.load().sf_linear8_bytes(M, K, N, x_code, W_code, needs, ctypes.byref(keep), ctypes.byref(temp),
+                                                ctypes.byref(later)))
+    return keep.value, temp.value, later.value
+
+
 def linear8_forward(x, W, b, needs):
     """(y, kept, backward's scratch bytes) of saeflow_b200.training.linear8: y = Q(x) @ Q(W) + b in x's dtype, and the
     buffer that its backward reads. needs: bits 1 dx, 2 dW, 4 db."""
@@ -251,16 +262,13 @@ def linear8_forward(x, W, b, needs):
     xm, wm = _abi.matrix(x, "x"), _abi.matrix(W, "W")
     bias = _vector(b, "b", N, dev)
     lib = _abi.load()
-    keep, temp, later = ctypes.c_size_t(0), ctypes.c_size_t(0), ctypes.c_size_t(0)
-    _abi.check(lib.sf_linear8_bytes(M, K, N, xm.dtype, wm.dtype, needs, ctypes.byref(keep), ctypes.byref(temp),
-                                    ctypes.byref(later)))
+    keep, temp, later = _linear8_bytes(M, K, N, xm.dtype, wm.dtype, needs, dev.index)
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
-    kept = torch.empty(keep.value, dtype=torch.uint8, device=dev) if keep.value else None
-    scratch = torch.empty(temp.value, dtype=torch.uint8, device=dev)
+    kept = torch.empty(keep, dtype=torch.uint8, device=dev) if keep else None
+    scratch = torch.empty(temp, dtype=torch.uint8, device=dev)
     _run(dev, lib.sf_linear8_forward, ctypes.byref(xm), ctypes.byref(wm), bias.data_ptr() if bias is not None else None,
-         ctypes.byref(_abi.matrix(y, "y")), needs, kept.data_ptr() if keep.value else None, scratch.data_ptr(),
-         temp.value)
-    return y, kept, later.value
+         ctypes.byref(_abi.matrix(y, "y")), needs, kept.data_ptr() if keep else None, scratch.data_ptr(), temp)
+    return y, kept, later
 
 
 def linear8_backward(dy, kept, K, x_dtype, W_dtype, needs, scratch_bytes):
