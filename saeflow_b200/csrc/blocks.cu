@@ -298,8 +298,10 @@ __device__ __forceinline__ void store_pair(__half *o, float a, float b) {
 // so piece c covers columns 8c - shift ... With shift = 0 a piece lies in one block; otherwise it may span
 // two, with two scales. Eight lanes take eight neighbouring pieces at a time and several times over, so
 // that enough bytes are on their way. `tile_shift` is 7 where a scale row serves 128 rows.
-// Bound by HBM: 16384 of 262144 rows of 2304 as bf16 in 17.9 us, 6.3 TB/s; as fp32 (four bytes written for one
-// read) 65536 rows in 140 us, 5.4 TB/s. Rows that start between boundaries: 5000 x 1001 fp16 10.5 us.
+// Bound by HBM: 16384 of 262144 rows of 2304 as bf16 in 18.5 us, 6.1 TB/s, with some of them still in L2, 22.0 us
+// with none; as fp32 (four bytes written for one read) 65536 rows in 140 us, 5.4 TB/s. Rows that start between
+// boundaries: 20000 x 777 bf16 17.8 us, 2.6 TB/s. Walking the rows with a grid that stays, each row's index
+// loaded a step ahead, was no faster (22.4 to 25.7 us).
 template <typename OT, bool ALIGNED>
 __global__ void __launch_bounds__(256, 4) read_rows_kernel(const uint8_t *__restrict__ q, int64_t q_pitch,
                                                         const uint8_t *__restrict__ s, int64_t s_pitch,
