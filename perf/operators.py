@@ -49,18 +49,17 @@ def listed():
         # one token against a 65536-feature dictionary: the weights' bytes
         {"name": "encode 1x2304x65536", "op": "encode", "rows": 1, "d": 2304, "features": 65536, "dtype": "bf16",
          "activation": "relu"},
-        # a short odd prompt and an SAE in fp32
-        {"name": "encode 100x768x16384 fp32", "op": "encode", "rows": 100, "d": 768, "features": 16384,
-         "dtype": "fp32", "activation": "relu"},
+        # a short odd prompt
+        {"name": "encode 100x768x16384", "op": "encode", "rows": 100, "d": 768, "features": 16384, "dtype": "bf16",
+         "activation": "relu"},
         # ragged in every extent, no activation
         {"name": "encode 3001x1000x24577", "op": "encode", "rows": 3001, "d": 1000, "features": 24577,
          "dtype": "fp16", "activation": "none"},
         # the benchmark's batch
         {"name": "encode 16384x2304x65536", "op": "encode", "rows": 16384, "d": 2304, "features": 65536,
          "dtype": "bf16", "activation": "relu"},
-        # a small ragged training step in fp32
-        {"name": "train 1000x768x5000 fp32", "op": "train", "rows": 1000, "d": 768, "features": 5000,
-         "dtype": "fp32"},
+        # a small ragged training step
+        {"name": "train 1000x768x5000", "op": "train", "rows": 1000, "d": 768, "features": 5000, "dtype": "bf16"},
         # a training step of a large dictionary
         {"name": "train 8192x2304x16384", "op": "train", "rows": 8192, "d": 2304, "features": 16384,
          "dtype": "bf16"},
@@ -83,7 +82,7 @@ def draw(rng):
         op = rng.choice(["write", "read", "encode", "train"])
         case = {"op": op, "rows": _size(rng, 1, 65536 if op in ("write", "read") else 16384, 64)}
         case["d"] = _size(rng, 64, 4608, 128)
-        case["dtype"] = rng.choice(["fp32", "bf16", "fp16"])
+        case["dtype"] = rng.choice(["fp32", "bf16", "fp16"] if op in ("write", "read") else ["bf16", "bf16", "fp16"])
         if op == "write":
             case["capacity"] = int(case["rows"] * rng.choice([1, 2, 4])) + rng.randrange(1000)
             case["slots"] = rng.choice(["run", "spread"])
