@@ -8,12 +8,22 @@
 // the instruction descriptor says which byte of the word applies. Tiles (one scale per 128 x 128) are
 // the same words read once per 128 rows.
 //
-// Persistent kernel, one CTA per SM, warp-specialised (352 threads):
+// Persistent kernel, one CTA per SM, warp-specialised (352 threads; 384 for long sums):
 //   warp 0      TMA producer: 128-byte rows of both operands, SWIZZLE_128B, mbarrier ring
 //   warp 1      TMEM allocator and MMA issuer
-//   warps 2-9   epilogue: bias, activation, rounding, stores; two warps to 32 rows, half the columns each
-//   warp 10     scale words of both operands for 512 elements of K into shared memory, in the order that
+//   8 warps     epilogue: bias, activation, rounding, stores; two warps to 32 rows, half the columns each
+//   1 warp      scale words of both operands for 512 elements of K into shared memory, in the order that
 //               tcgen05.cp spreads over TMEM (row r at byte 16 (r % 32) + 4 (r / 32))
+//
+// Long sums (RANGES). The tensor cores add 32 products at a time to the sum in TMEM and round it toward zero, a
+// bias that grows with the number of additions. So a sum stays in TMEM for a range of K, at most 1024 for fp32
+// outputs and 2560 for 16-bit ones, and the epilogue warps add the ranges in registers, rounding to nearest.
+// Error against 64 bits (relative, 4096 x K x 4096; one range / these / an fp32 FMA chain): operands of both signs
+// K = 2304 1.2e-7 / 6.4e-8 / 6.2e-8, 8192 4.9e-7 / 8.1e-8 / 1.3e-7; of one sign 2304 6.1e-7 / 1.7e-7 / 1.3e-7, 8192
+// 3.9e-6 / 1.9e-7 / 4.3e-7. Of 16-bit outputs (bf16, K = 2304 to 16384) one number in ten thousand rounds to the
+// neighbour of the exact one's, as with an fp32 chain; ranges of 1024 would halve that. A handoff between two ranges
+// takes about 1000 clocks (a range of 1024 about 5000): 4096 x 2304 x 16384 fp32 154 -> 175 us, 2304 x 8192 x 16384
+// bf16 246 -> 281 us, 8192 x 16384 x 2304 bf16 279 -> 276 us, against one range each.
 //
 // Two sizes. PAIR: a CTA pair (cta_group::2) computes 256 x 256, each CTA loading 128 rows of either
 // operand; both CTAs' loads complete on the leader's barriers. Single: one CTA computes 128 x COLS.
@@ -42,7 +52,11 @@ namespace {
 constexpr int kKBytes = 128;                   // elements (bytes) of K per stage
 constexpr int kScaleSlots = 3;                 // scale words of 512 elements of K each
 constexpr int kEpilogueWarps = 8;              // two for each quarter of the TMEM lanes
-constexpr int kThreads = 32 * (3 + kEpilogueWarps);
+// Long sums (RANGES) keep 128 more registers in each epilogue thread, which the four warps before them give up:
+// 128 x 56 + 256 x 224 = 384 x 168, what the block is launched with.
+constexpr int threads_of(bool ranges) { return 32 * ((ranges ? 4 : 3) + kEpilogueWarps); }
+constexpr int kControlRegs = 56, kEpilogueRegs = 224, kLaunchRegs = 168;
+static_assert(128 * kControlRegs + 32 * kEpilogueWarps * kEpilogueRegs == threads_of(true) * kLaunchRegs, "registers");
 constexpr int kTmemCols = 512;
 constexpr int kPairCols = 256;                 // columns of a pair's tile
 constexpr int kRowTile = 128;                  // rows (TMEM lanes) per CTA
@@ -51,6 +65,7 @@ struct GemmParams {
     int rows, cols;            // of the tile grid: a's and b's, or b's and a's (kSwapped)
     int nkb, groups;           // K blocks of 128, and groups of four of them
     int splits, split_groups;  // ranges of K: split z takes groups [z split_groups, (z + 1) split_groups)
+    int range_groups;          // groups whose sum the tensor cores keep; ranges are added in fp32 registers (RANGES)
     int row_tiles, col_tiles;
     int col_bytes;             // the columns' operand per CTA and stage, as its TMA box is cut
     int group_rows;            // row tiles that run side by side over each column tile
@@ -299,8 +314,8 @@ __device__ __forceinline__ void store_runs(const uint8_t *buf, OT *out, int64_t 
     }
 }
 
-template <typename OT, typename S, int STORE>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename OT, typename S, int STORE, bool RANGES>
+__global__ void __launch_bounds__(threads_of(RANGES), 1)
     block_gemm_kernel(const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmC,
                       const __grid_constant__ CUtensorMap tmOut, const GemmParams p) {
     constexpr bool PAIR = S::PAIR, SWAP = STORE == kSwapped;
@@ -313,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *sScale = sOut + kEpilogueWarps * OUT_BYTES;
     Shared *sh = reinterpret_cast<Shared *>(sScale + kScaleSlots * S::SLOT_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int EPI = RANGES ? 4 : 2;  // the first epilogue warp; the scales' is the last, or (RANGES) the third
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
     const bool leader = rank == 0;
     const int first_unit = PAIR ? (int)cluster_id_x() : (int)blockIdx.x;
@@ -401,140 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
 
-    if (warp == 0) {
-        // ---------------------------------------------------------------- TMA producer
-        if (lane == 0) {
-            // a group's row tiles are read again for each of its column tiles
-            const uint64_t pol_c = l2_policy_evict_normal();
-            const uint64_t pol_r = p.col_tiles > 1 ? l2_policy_evict_last() : pol_c;
-            int stage = 0;
-            uint32_t phase = 0, armed = 0, armed_parity = 0;
-            bool ok = true;
-            for (int u = first_unit; ok && u < units; u += step_units) {
-                const Unit un = unit_of<S>(p, u);
-                const int row0 = un.row0 + (int)rank * kRowTile, col0 = un.col0 + (int)rank * S::COLS_HERE;
-                for (int kb = un.kb0; kb < un.kb1; ++kb) {
-                    if (!(ok = wait(&sh->empty[stage], phase ^ 1u))) break;
-                    if (leader) {
-                        mbar_arrive_expect_tx(&sh->full[stage], kCtas * (S::R_BYTES + p.col_bytes));
-                        armed |= 1u << stage;
-                        armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-                    }
-                    uint8_t *dr = sR + stage * S::R_BYTES, *dc = sC + stage * S::C_BYTES;
-                    if (PAIR) {
-                        const uint32_t full = map_to_rank(smem_u32(&sh->full[stage]), 0);
-                        tma_load_2d_pair(dr, &tmR, full, kb * kKBytes, row0, pol_r);
-                        tma_load_2d_pair(dc, &tmC, full, kb * kKBytes, col0, pol_c);
-                    } else {
-                        tma_load_2d(dr, &tmR, &sh->full[stage], kb * kKBytes, row0, pol_r);
-                        tma_load_2d(dc, &tmC, &sh->full[stage], kb * kKBytes, col0, pol_c);
-                    }
-                    if (++stage == S::STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                }
-            }
-            if (*abort_flag) {  // copies in flight must land before the CTA leaves
-                if (leader) {
-                    for (int s = 0; s < S::STAGES; ++s)
-                        if (armed & (1u << s)) mbar_wait_drain(&sh->full[s], (armed_parity >> s) & 1u, p.err);
-                } else {
-                    const unsigned long long t0 = global_timer_ns();
-                    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // ---------------------------------------------------------------- MMA issuer (the leader's)
-        // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers, and
-        // one elected lane issues: with the loop inside a one-lane branch each instruction's operands were
-        // moved there one by one (some 140 clocks an MMA, more than a 256 x 256 x 32 one takes).
-        if (leader) {
-            const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-            const uint64_t desc_r = smem_desc_sw128(smem_u32(sR), 16, 1024);
-            const uint64_t desc_c = smem_desc_sw128(smem_u32(sC), 16, 1024);
-            const uint64_t desc_s = smem_desc_rows16(smem_u32(sScale));
-            int stage = 0, slot = 0, acc = 0;
-            uint32_t phase = 0, slot_phase = 0, acc_phase = 0;
-            bool ok = true, first_tile = true;
-            for (int u = first_unit; ok && u < units; u += step_units) {
-                const Unit un = unit_of<S>(p, u);
-                // Accumulators that overlap: the previous tile's epilogue must have read the columns that
-                // this tile's shares with it (and so has finished the tile before that).
-                if (S::OVERLAP) {
-                    if (!first_tile && !(ok = wait_warp(&sh->tmem_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1u))) break;
-                    first_tile = false;
-                } else if (!(ok = wait_warp(&sh->tmem_empty[acc], acc_phase ^ 1u))) {
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d = tmem_u + acc * S::ACC1;
-                for (int kb4 = un.kb0; ok && kb4 < un.kb1; kb4 += 4) {
-                    if (!(ok = wait_warp_cluster(&sh->scale_full[slot], slot_phase))) break;
-                    tc_fence_after();
-                    const uint32_t scales = tmem_u + S::SCALE_COL + slot * S::SLOT_COLS;
-                    if (elect_one()) {
-                        const uint64_t src = desc_s + slot * (S::SLOT_BYTES >> 4);
-#pragma unroll
-                        for (int i = 0; i < S::SLOT_COLS / 4; ++i) {
-                            if (PAIR)
-                                tmem_copy_32x128b_pair(scales + 4 * i, src + 32 * i);
-                            else
-                                tmem_copy_32x128b(scales + 4 * i, src + 32 * i);
-                        }
-                    }
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (kb4 + j >= un.kb1) break;
-                        if (!(ok = wait_warp(&sh->full[stage], phase))) break;
-                        tc_fence_after();
-                        const uint64_t rd = desc_r + stage * (S::R_BYTES >> 4), cd = desc_c + stage * (S::C_BYTES >> 4);
-                        constexpr uint32_t IDESC0 = make_idesc_e4m3_scaled(S::ROWS, S::COLS, 0);
-                        const uint32_t idesc = IDESC0 | (j << 4) | (j << 29);
-                        if (elect_one()) {
-#pragma unroll
-                            for (int ks = 0; ks < 4; ++ks) {
-                                const uint32_t accumulate = (kb4 > un.kb0 || j || ks) ? 1u : 0u;
-                                if (PAIR)
-                                    umma_e4m3_scaled_pair(d, rd + 2 * ks, cd + 2 * ks, idesc, scales, scales + 4,
-                                                          accumulate);
-                                else
-                                    umma_e4m3_scaled(d, rd + 2 * ks, cd + 2 * ks, idesc, scales, scales + 4, accumulate);
-                            }
-                            commit(&sh->empty[stage]);
-                            // Released with the group's last MMA: a slot is filled again, in shared memory and
-                            // then in TMEM, only after the MMAs that read it.
-                            if (j == 3 || kb4 + j + 1 == un.kb1) commit(&sh->scale_empty[slot]);
-                            if (kb4 + j + 1 == un.kb1) commit(&sh->tmem_full[acc]);
-                        }
-                        __syncwarp();
-                        if (++stage == S::STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
-                    }
-                    if (++slot == kScaleSlots) {
-                        slot = 0;
-                        slot_phase ^= 1u;
-                    }
-                }
-                if (++acc == 2) {
-                    acc = 0;
-                    acc_phase ^= 1u;
-                }
-            }
-            if (elect_one()) {
-                if (PAIR)
-                    umma_commit_pair(map_to_rank(smem_u32(&sh->drain), 0));
-                else
-                    umma_commit(&sh->drain);
-            }
-            __syncwarp();
-            mbar_wait_drain(&sh->drain, 0, p.err);
-        }
-    } else if (warp < 2 + kEpilogueWarps) {
+    if (warp >= EPI && warp < EPI + kEpilogueWarps) {
+        if (RANGES) set_registers_up<kEpilogueRegs>();
         // ---------------------------------------------------------------- epilogue
         const int quad = warp & 3;
         // This warp's columns: a half of the tile's, or the first warp all 32 of the narrowest.
@@ -542,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int STEP = HALF < 64 ? HALF : 64;  // columns loaded at a time
         constexpr int STEPS = HALF / STEP;
         static_assert(STEPS <= 2, "at most two steps a tile");
-        const int half = (warp - 2) >> 2;
+        static_assert(S::OVERLAP || STEPS == 1, "released after the first step");
+        const int half = (warp - EPI) >> 2;
         const bool mine = half * HALF < S::COLS;
         int acc = 0;
         uint32_t acc_phase = 0;
@@ -550,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // this warp's columns, passed through the warp's own shared memory (no barrier between warps).
         constexpr int OWN = SWAP ? 1 : HALF / 32;
         float next_bias[OWN], next_thr[OWN];
-        float *my_bias = sh->bias[warp - 2], *my_thr = sh->thr[warp - 2];
+        float *my_bias = sh->bias[warp - EPI], *my_thr = sh->thr[warp - EPI];
         auto load_vectors = [&](const Unit &un) {
 #pragma unroll
             for (int j = 0; j < OWN; ++j) {
@@ -577,19 +462,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             next = unit_of<S>(p, min(u + step_units, units - 1));
             load_vectors(next);
-            if (!wait_warp(&sh->tmem_full[acc], acc_phase)) break;
+            if (!RANGES && !wait_warp(&sh->tmem_full[acc], acc_phase)) break;
             tc_fence_after();
-            const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * S::ACC1 + half * HALF;
+            const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * HALF;
             // Overlapping accumulators: the shared columns (the first's last 40, the second's first 40) are
             // read first and released to the next tile's MMAs. A warp whose half has none of them releases at
             // once: what it still had to read of the tile before, in the accumulator that those MMAs take, it has.
-            const bool shares = !S::OVERLAP || half == (acc ^ 1);
             auto release = [&]() {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) release_leader(&sh->tmem_empty[acc]);
             };
-            if (!shares || !mine) release();
+            auto advance = [&]() {
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            };
 
             // Columns [c0, c0 + STEP) of this warp's half, from r to the output.
             auto put = [&](uint32_t (&r)[STEP / 32][32], int c0, bool last) {
@@ -613,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         finish32<OT>(
                             r[h], p.activation, [&](int j) { return *reinterpret_cast<const float4 *>(my_bias + c + j); },
                             [&](int j) { return my_thr[c + j]; }, o);
-                        uint8_t *buf = sOut + (warp - 2) * OUT_BYTES;
+                        uint8_t *buf = sOut + (warp - EPI) * OUT_BYTES;
                         const int row_w = un.row0 + (int)rank * kRowTile + quad * 32;
                         constexpr int CHUNKS = 2 * sizeof(OT);
                         if constexpr (STORE == kTma) {
@@ -663,65 +552,261 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             };
-            // One step's sums at a time: loading the second while the first is finished spilled registers, and
-            // was slower at every size measured (16384 x 256 x 65536: 773 against 638 us).
-            const int c_first = STEPS == 2 && acc == 0 ? STEP : 0;
-#pragma unroll 1
-            for (int i = 0; mine && i < STEPS; ++i) {
-                const int c0 = i == 0 ? c_first : STEP - c_first;
-                uint32_t r[STEP / 32][32];
+            if constexpr (RANGES) {
+                // Long K: the sums of its ranges, added here in their order with rounding to nearest.
+                float sums[STEPS][STEP / 32][32];
 #pragma unroll
-                for (int h = 0; h < STEP / 32; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
-                tmem_ld_wait();
-                if (shares && i == (S::OVERLAP ? 0 : STEPS - 1)) release();
-                put(r, c0, i == STEPS - 1);
-            }
-            if (++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1u;
+                for (int i = 0; i < STEPS * STEP; ++i) sums[i / STEP][i % STEP / 32][i % 32] = 0.f;
+                bool ok = true;
+                for (int kb0 = un.kb0; kb0 < un.kb1; kb0 += 4 * p.range_groups) {
+                    if (!(ok = wait_warp(&sh->tmem_full[acc], acc_phase))) break;
+                    tc_fence_after();
+                    const bool shares = !S::OVERLAP || half == (acc ^ 1);
+                    if (!shares || !mine) release();
+                    uint32_t r[STEP / 32][32];
+                    auto load = [&](int i) {
+#pragma unroll
+                        for (int h = 0; h < STEP / 32; ++h)
+                            tmem_ld_32x32b_x32(lanes + acc * S::ACC1 + i * STEP + 32 * h, r[h]);
+                        tmem_ld_wait();
+                    };
+                    auto add = [&](int i) {
+#pragma unroll
+                        for (int j = 0; j < STEP; ++j) {
+                            sums[i][j / 32][j % 32] += __uint_as_float(r[j / 32][j % 32]);
+                            asm volatile("" : "+f"(sums[i][j / 32][j % 32]));  // before the next load: else both are held
+                        }
+                    };
+                    if (mine) {
+                        if (STEPS == 2 && acc == 0) {
+                            load(STEPS - 1);
+                            if (shares) release();
+                            add(STEPS - 1);
+                            load(0);
+                            add(0);
+                        } else {
+                            load(0);
+                            if (shares) release();
+                            add(0);
+                            if (STEPS == 2) {
+                                load(STEPS - 1);
+                                add(STEPS - 1);
+                            }
+                        }
+                    }
+                    advance();
+                }
+                if (!ok) break;
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < STEPS; ++i) {
+                        uint32_t r[STEP / 32][32];
+#pragma unroll
+                        for (int j = 0; j < STEP; ++j) r[j / 32][j % 32] = __float_as_uint(sums[i][j / 32][j % 32]);
+                        put(r, i * STEP, i == STEPS - 1);
+                    }
+                }
+            } else {
+                const bool shares = !S::OVERLAP || half == (acc ^ 1);
+                const uint32_t taddr = lanes + acc * S::ACC1;
+                if (!shares || !mine) release();
+                // One step's sums at a time: loading the second while the first is finished spilled registers, and
+                // was slower at every size measured (16384 x 256 x 65536: 773 against 638 us).
+                const int c_first = STEPS == 2 && acc == 0 ? STEP : 0;
+#pragma unroll 1
+                for (int i = 0; mine && i < STEPS; ++i) {
+                    const int c0 = i == 0 ? c_first : STEP - c_first;
+                    uint32_t r[STEP / 32][32];
+#pragma unroll
+                    for (int h = 0; h < STEP / 32; ++h) tmem_ld_32x32b_x32(taddr + c0 + 32 * h, r[h]);
+                    tmem_ld_wait();
+                    if (shares && i == (S::OVERLAP ? 0 : STEPS - 1)) release();
+                    put(r, c0, i == STEPS - 1);
+                }
+                advance();
             }
         }
         if (STORE == kTma) tma_store_wait_read<0>();  // the buffers go with the CTA
     } else {
-        // ---------------------------------------------------------------- scales (both CTAs)
-        // A group's words are loaded while the one before waits for its slot: a load from HBM takes as long
-        // as the MMAs of a group.
-        constexpr int WORDS = 1 + S::COL_WORDS / 4;
-        int u = first_unit, g = 0;
-        Unit un = unit_of<S>(p, u < units ? u : 0);
-        g = un.kb0 / 4;
-        uint4 w[WORDS];
-        auto load = [&]() {
-            w[0] = scale_words(p.r_scales, p.r_pitch, p.r_shift, un.row0 + (int)rank * kRowTile, p.rows, g, lane);
-#pragma unroll
-            for (int i = 1; i < WORDS; ++i)
-                w[i] = scale_words(p.c_scales, p.c_pitch, p.c_shift, un.col0 + 128 * (i - 1), p.cols, g, lane);
-        };
-        int slot = 0;
-        uint32_t phase = 0;
-        if (u < units) load();
-        while (u < units) {
-            uint4 now[WORDS];
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) now[i] = w[i];
-            if (4 * ++g >= un.kb1) {
-                u += step_units;
-                if (u < units) {
-                    un = unit_of<S>(p, u);
-                    g = un.kb0 / 4;
+        if (RANGES) set_registers_down<kControlRegs>();
+        if (warp == 0) {
+            // ---------------------------------------------------------------- TMA producer
+            if (lane == 0) {
+                // a group's row tiles are read again for each of its column tiles
+                const uint64_t pol_c = l2_policy_evict_normal();
+                const uint64_t pol_r = p.col_tiles > 1 ? l2_policy_evict_last() : pol_c;
+                int stage = 0;
+                uint32_t phase = 0, armed = 0, armed_parity = 0;
+                bool ok = true;
+                for (int u = first_unit; ok && u < units; u += step_units) {
+                    const Unit un = unit_of<S>(p, u);
+                    const int row0 = un.row0 + (int)rank * kRowTile, col0 = un.col0 + (int)rank * S::COLS_HERE;
+                    for (int kb = un.kb0; kb < un.kb1; ++kb) {
+                        if (!(ok = wait(&sh->empty[stage], phase ^ 1u))) break;
+                        if (leader) {
+                            mbar_arrive_expect_tx(&sh->full[stage], kCtas * (S::R_BYTES + p.col_bytes));
+                            armed |= 1u << stage;
+                            armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
+                        }
+                        uint8_t *dr = sR + stage * S::R_BYTES, *dc = sC + stage * S::C_BYTES;
+                        if (PAIR) {
+                            const uint32_t full = map_to_rank(smem_u32(&sh->full[stage]), 0);
+                            tma_load_2d_pair(dr, &tmR, full, kb * kKBytes, row0, pol_r);
+                            tma_load_2d_pair(dc, &tmC, full, kb * kKBytes, col0, pol_c);
+                        } else {
+                            tma_load_2d(dr, &tmR, &sh->full[stage], kb * kKBytes, row0, pol_r);
+                            tma_load_2d(dc, &tmC, &sh->full[stage], kb * kKBytes, col0, pol_c);
+                        }
+                        if (++stage == S::STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+                if (*abort_flag) {  // copies in flight must land before the CTA leaves
+                    if (leader) {
+                        for (int s = 0; s < S::STAGES; ++s)
+                            if (armed & (1u << s)) mbar_wait_drain(&sh->full[s], (armed_parity >> s) & 1u, p.err);
+                    } else {
+                        const unsigned long long t0 = global_timer_ns();
+                        while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+                    }
                 }
             }
-            if (u < units) load();
-            if (!wait_warp(&sh->scale_empty[slot], phase ^ 1u)) break;
-            uint8_t *dst = sScale + slot * S::SLOT_BYTES + lane * 16;
+        } else if (warp == 1) {
+            // ---------------------------------------------------------------- MMA issuer (the leader's)
+            // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers, and
+            // one elected lane issues: with the loop inside a one-lane branch each instruction's operands were
+            // moved there one by one (some 140 clocks an MMA, more than a 256 x 256 x 32 one takes).
+            if (leader) {
+                const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+                const uint64_t desc_r = smem_desc_sw128(smem_u32(sR), 16, 1024);
+                const uint64_t desc_c = smem_desc_sw128(smem_u32(sC), 16, 1024);
+                const uint64_t desc_s = smem_desc_rows16(smem_u32(sScale));
+                int stage = 0, slot = 0, acc = 0;
+                uint32_t phase = 0, slot_phase = 0, acc_phase = 0;
+                bool ok = true, first = true;
+                for (int u = first_unit; ok && u < units; u += step_units) {
+                    const Unit un = unit_of<S>(p, u);
+                    // A sum in TMEM runs over a range of K, the whole of the unit's unless it is long (RANGES).
+                    for (int kb0 = un.kb0; ok && kb0 < un.kb1; kb0 += RANGES ? 4 * p.range_groups : un.kb1) {
+                        const int kb1 = RANGES ? min(un.kb1, kb0 + 4 * p.range_groups) : un.kb1;
+                        // Accumulators that overlap: the previous sum's epilogue must have read the columns that
+                        // this one shares with it (and so has finished the sum before that).
+                        if (S::OVERLAP) {
+                            if (!first && !(ok = wait_warp(&sh->tmem_empty[acc ^ 1], acc ? acc_phase : acc_phase ^ 1u))) break;
+                            first = false;
+                        } else if (!(ok = wait_warp(&sh->tmem_empty[acc], acc_phase ^ 1u))) {
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t d = tmem_u + acc * S::ACC1;
+                        for (int kb4 = kb0; ok && kb4 < kb1; kb4 += 4) {
+                            if (!(ok = wait_warp_cluster(&sh->scale_full[slot], slot_phase))) break;
+                            tc_fence_after();
+                            const uint32_t scales = tmem_u + S::SCALE_COL + slot * S::SLOT_COLS;
+                            if (elect_one()) {
+                                const uint64_t src = desc_s + slot * (S::SLOT_BYTES >> 4);
 #pragma unroll
-            for (int i = 0; i < WORDS; ++i) *reinterpret_cast<uint4 *>(dst + 512 * i) = now[i];
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) arrive_leader(&sh->scale_full[slot]);
-            if (++slot == kScaleSlots) {
-                slot = 0;
-                phase ^= 1u;
+                                for (int i = 0; i < S::SLOT_COLS / 4; ++i) {
+                                    if (PAIR)
+                                        tmem_copy_32x128b_pair(scales + 4 * i, src + 32 * i);
+                                    else
+                                        tmem_copy_32x128b(scales + 4 * i, src + 32 * i);
+                                }
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (kb4 + j >= kb1) break;
+                                if (!(ok = wait_warp(&sh->full[stage], phase))) break;
+                                tc_fence_after();
+                                const uint64_t rd = desc_r + stage * (S::R_BYTES >> 4), cd = desc_c + stage * (S::C_BYTES >> 4);
+                                constexpr uint32_t IDESC0 = make_idesc_e4m3_scaled(S::ROWS, S::COLS, 0);
+                                const uint32_t idesc = IDESC0 | (j << 4) | (j << 29);
+                                if (elect_one()) {
+#pragma unroll
+                                    for (int ks = 0; ks < 4; ++ks) {
+                                        const uint32_t accumulate = (kb4 > kb0 || j || ks) ? 1u : 0u;
+                                        if (PAIR)
+                                            umma_e4m3_scaled_pair(d, rd + 2 * ks, cd + 2 * ks, idesc, scales, scales + 4,
+                                                                  accumulate);
+                                        else
+                                            umma_e4m3_scaled(d, rd + 2 * ks, cd + 2 * ks, idesc, scales, scales + 4, accumulate);
+                                    }
+                                    commit(&sh->empty[stage]);
+                                    // Released with the group's last MMA: a slot is filled again, in shared memory and
+                                    // then in TMEM, only after the MMAs that read it.
+                                    if (j == 3 || kb4 + j + 1 == kb1) commit(&sh->scale_empty[slot]);
+                                    if (kb4 + j + 1 == kb1) commit(&sh->tmem_full[acc]);
+                                }
+                                __syncwarp();
+                                if (++stage == S::STAGES) {
+                                    stage = 0;
+                                    phase ^= 1u;
+                                }
+                            }
+                            if (++slot == kScaleSlots) {
+                                slot = 0;
+                                slot_phase ^= 1u;
+                            }
+                        }
+                        if (++acc == 2) {
+                            acc = 0;
+                            acc_phase ^= 1u;
+                        }
+                    }
+                }
+                if (elect_one()) {
+                    if (PAIR)
+                        umma_commit_pair(map_to_rank(smem_u32(&sh->drain), 0));
+                    else
+                        umma_commit(&sh->drain);
+                }
+                __syncwarp();
+                mbar_wait_drain(&sh->drain, 0, p.err);
+            }
+        } else if (!RANGES || warp == 2) {
+            // ---------------------------------------------------------------- scales (both CTAs)
+            // A group's words are loaded while the one before waits for its slot: a load from HBM takes as long
+            // as the MMAs of a group.
+            constexpr int WORDS = 1 + S::COL_WORDS / 4;
+            int u = first_unit, g = 0;
+            Unit un = unit_of<S>(p, u < units ? u : 0);
+            g = un.kb0 / 4;
+            uint4 w[WORDS];
+            auto load = [&]() {
+                w[0] = scale_words(p.r_scales, p.r_pitch, p.r_shift, un.row0 + (int)rank * kRowTile, p.rows, g, lane);
+#pragma unroll
+                for (int i = 1; i < WORDS; ++i)
+                    w[i] = scale_words(p.c_scales, p.c_pitch, p.c_shift, un.col0 + 128 * (i - 1), p.cols, g, lane);
+            };
+            int slot = 0;
+            uint32_t phase = 0;
+            if (u < units) load();
+            while (u < units) {
+                uint4 now[WORDS];
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) now[i] = w[i];
+                if (4 * ++g >= un.kb1) {
+                    u += step_units;
+                    if (u < units) {
+                        un = unit_of<S>(p, u);
+                        g = un.kb0 / 4;
+                    }
+                }
+                if (u < units) load();
+                if (!wait_warp(&sh->scale_empty[slot], phase ^ 1u)) break;
+                uint8_t *dst = sScale + slot * S::SLOT_BYTES + lane * 16;
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) *reinterpret_cast<uint4 *>(dst + 512 * i) = now[i];
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&sh->scale_full[slot]);
+                if (++slot == kScaleSlots) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
             }
         }
     }
@@ -775,7 +860,8 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const float *__restric
 template <typename OT, typename S, int STORE>
 int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tmOut, const GemmParams &p,
            cudaStream_t stream) {
-    auto kern = block_gemm_kernel<OT, S, STORE>;
+    const bool ranges = p.range_groups < p.split_groups;
+    auto kern = ranges ? block_gemm_kernel<OT, S, STORE, true> : block_gemm_kernel<OT, S, STORE, false>;
     constexpr size_t smem = 1024 + S::STAGES * (S::R_BYTES + S::C_BYTES) + kEpilogueWarps * out_bytes(STORE) +
                             kScaleSlots * S::SLOT_BYTES + sizeof(Shared);
     static_assert(smem <= 232448, "shared memory per block");
@@ -784,7 +870,7 @@ int launch(const CUtensorMap &tmR, const CUtensorMap &tmC, const CUtensorMap &tm
     const int units = p.row_tiles * p.col_tiles * p.splits;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads_of(ranges));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
@@ -815,7 +901,8 @@ using One128 = Shape<false, 128, 6>;
 struct Plan {
     bool pair;   // CTA pairs on 256 x 256 tiles; else single CTAs on 128 rows of b x `cols` rows of a (kSwapped)
     int cols;
-    int splits;  // ranges of K
+    int splits;  // of K, among SMs and into a workspace
+    int range_groups;  // groups of 512 of K to a sum in TMEM
 };
 
 int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -840,12 +927,13 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int out_dtype) {
     // second kernel. Measured (us, split against whole): K = 768 12.7 / 9.5 (512 x 2048), 2304 13.0 / 12.4
     // (256 x 2048), 5000 19.3 / 23.6 (1000 x 768), 8192 16.1 / 24.4 (640 x 640), 13558 23.5 / 35.1 (636 x 1094).
     pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(groups / 4, slots / tiles));
-    // The tensor cores round each addition toward zero, a bias that grows with the number of additions
-    // (measured against 64 bits: 9e-7 of the result at K = 8192, 1.2e-5 at 65536), far below a 16-bit
-    // output's rounding but not an fp32 one's: those sum ranges of at most 8192, joined in fp32.
+    // fp32 outputs: splits of at most 8192, whatever the number of tiles.
     if (out_dtype == SF_F32) pl.splits = std::max(pl.splits, cdiv(K, 8192));
-    // whole ranges: no split without a group
-    pl.splits = cdiv(groups, cdiv(groups, pl.splits));
+    // whole splits: none without a group
+    const int split_groups = cdiv(groups, pl.splits);
+    pl.splits = cdiv(groups, split_groups);
+    const int most = out_dtype == SF_F32 ? 2 : 5;  // 1024 or 2560 of K: the errors are at the top of this file
+    pl.range_groups = cdiv(split_groups, cdiv(split_groups, most));
     return pl;
 }
 
@@ -939,6 +1027,7 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     p.groups = cdiv(p.nkb, 4);
     p.splits = pl.splits;
     p.split_groups = cdiv(p.groups, pl.splits);
+    p.range_groups = pl.range_groups;
     p.row_tiles = cdiv(p.rows, row_tile);
     p.col_tiles = cdiv(p.cols, pl.cols);
     // A group of row tiles runs side by side over each column tile: the columns' operand is read from HBM

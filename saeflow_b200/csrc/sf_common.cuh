@@ -114,6 +114,16 @@ __device__ __forceinline__ bool elect_one() {
     return pred != 0;
 }
 
+// A warpgroup's registers per thread, given up or taken on; all of its threads run it.
+template <int N>
+__device__ __forceinline__ void set_registers_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_registers_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ---------------------------------------------------------------------------------------
 // mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {

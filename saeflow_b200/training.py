@@ -132,7 +132,7 @@ def linear8(x, W, b=None):
 
     x [M, K], W [K, N] (the orientation of W_enc and W_dec), b [N] or None; fp32 / bf16 / fp16. Every
     product is of operands quantised to e4m3 with a power-of-two scale per block of 128 along the axis
-    it sums over (W: per 128 x 128 tile), accumulated in fp32, rounded once to the dtype of what it
+    it sums over (W: per 128 x 128 tile), accumulated in fp32 as block_matmul says, rounded once to the dtype of what it
     computes (y and dx: x's, dW: W's):
         y  = Q(x) @ Q(W) + b        dx = Q(dy) @ Q(W)^T
         dW = Q(x^T) @ Q(dy^T)^T     db = sum_rows dy   (dy as it is, fp32, in a fixed order)
