@@ -958,10 +958,12 @@ int check_product(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out) 
     return SF_OK;
 }
 
-// Rows that TMA can write: 16-byte aligned base and pitch.
+// Rows that TMA can write: 16-byte aligned base, pitch and length. A store of a row that ends between boundaries
+// writes up to the next one (measured: zeros beside the output, in every type).
 bool tma_rows(const sf_matrix &out) {
+    const int64_t es = (int64_t)dtype_size(out.dtype);
     return reinterpret_cast<uintptr_t>(out.data) % 16 == 0 && out.stride_row >= out.cols &&
-           (out.stride_row * (int64_t)dtype_size(out.dtype)) % 16 == 0;
+           (out.stride_row * es) % 16 == 0 && (out.cols * es) % 16 == 0;
 }
 
 template <typename OT>
@@ -1015,7 +1017,7 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     if (partial) {
         dst.data = workspace;
         dst.dtype = SF_F32;
-        dst.stride_row = partial_pitch(N);
+        dst.stride_row = dst.cols = partial_pitch(N);  // whole 16-byte units: what is past column N is not read
     }
     const int store = !pl.pair ? kSwapped : tma_rows(dst) ? kTma : kRows;
     const sf_blocks *R = pl.pair ? a : b, *C = pl.pair ? b : a;
@@ -1061,7 +1063,7 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
         return st;
     const int64_t es = (int64_t)dtype_size(dst.dtype);
     if (store == kTma &&
-        (st = make_map_out(&tmOut, dst.data, dst.dtype, (uint64_t)N, (uint64_t)M, (uint64_t)pl.splits,
+        (st = make_map_out(&tmOut, dst.data, dst.dtype, (uint64_t)dst.cols, (uint64_t)M, (uint64_t)pl.splits,
                            (uint64_t)(dst.stride_row * es), (uint64_t)(p.out_split * es))))
         return st;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -247,7 +247,8 @@ __device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *m
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "l"(l2_policy)
         : "memory");
 }
-// TMA store of a box from shared memory; elements past the tensor's extents are not written.
+// TMA store of a box from shared memory; what is past the tensor's extents is not written, but for the rest of a
+// 16-byte unit that holds the last column: rows are a whole number of units.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *smem_src, int32_t c0, int32_t c1,
                                              int32_t c2) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(

@@ -11,7 +11,7 @@ nearest, whose errors have no sign.
 import pytest
 import torch
 
-from saeflow_b200.kernels import block_matmul, device_error, quantize
+from saeflow_b200.kernels import BlockScaled, block_matmul, device_error, quantize
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,33 @@ def test_long_16_bit_sums_round_as_the_exact_ones(M, N, dtype):
     got = block_matmul(a8, b8, out_dtype=dtype)
     share = (got != want).double().mean().item()
     assert share <= 80 * 2.0 ** -25 / SPACING[dtype], f"{share:.3g} of the sums round to a neighbour"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(1000, 3001, 640), (2500, 4101, 130), (1100, 2902, 2700), (40, 1003, 300)])
+def test_nothing_beside_an_output_is_written(M, N, K, dtype):
+    """Columns of wider memory whose rows start on 16-byte boundaries and end between them."""
+    a8, b8, want = one_sign(M, N, K)
+    wide = torch.full((M, 4400), 7.0, dtype=dtype, device="cuda")
+    got = block_matmul(a8, b8, out=wide[:, 16:16 + N])
+    assert (wide[:, :16] == 7).all() and (wide[:, 16 + N:] == 7).all()
+    assert torch.allclose(got.double(), want, rtol=2 * SPACING.get(dtype, 2.0 ** -19))
+    assert torch.equal(got, block_matmul(a8, b8, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("M,N,K", [(1000, 3000, 301), (100, 700, 130), (7, 300, 1)])
+def test_nothing_beside_an_operand_is_read(M, N, K):
+    """Operands that are columns of wider memory, NaN numbers and NaN scales on both sides of them."""
+    a8, b8, want = one_sign(M, N, K)
+
+    def wide(q):
+        data = torch.full((q.shape[0] + 3, K + 150), 0x7F, dtype=torch.uint8, device="cuda")
+        data = data[:, :(K + 150) // 16 * 16].contiguous()[:, 32:32 + K]
+        data[:q.shape[0]] = q.data.view(torch.uint8)
+        scales = torch.full((q.scales.shape[0] + 3, 16), 0xFF, dtype=torch.uint8, device="cuda")[:, 4:4 + q.scales.shape[1]]
+        scales[:q.scales.shape[0]] = q.scales
+        return BlockScaled(data[:q.shape[0]].view(torch.float8_e4m3fn), scales[:q.scales.shape[0]], q.tile)
+
+    got = block_matmul(wide(a8), wide(b8), out_dtype=torch.float32)
+    assert torch.equal(got, block_matmul(a8, b8, out_dtype=torch.float32)) and torch.isfinite(got).all()
+    assert torch.allclose(got.double(), want, rtol=2.0 ** -18)
