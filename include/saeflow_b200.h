@@ -370,6 +370,17 @@ SF_API int sf_blocks_quantize(const sf_matrix *x, const sf_blocks *q, const sf_b
 SF_API int sf_block_matmul_workspace(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out, size_t *bytes);
 
 /*
+ * How sf_block_matmul computes this product: tile_rows x tile_cols of out per tile (256 x 256: a CTA pair; else
+ * one CTA on 128 features), in how many splits of K, joined from the workspace, and how much of K a sum in the
+ * tensor cores runs over.
+ */
+typedef struct sf_block_plan {
+    int32_t tile_rows, tile_cols;
+    int32_t splits, range;
+} sf_block_plan;
+SF_API int sf_block_matmul_plan(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out, sf_block_plan *plan);
+
+/*
  * out = act(a @ b^T + bias): a [M, K] and b [N, K], each in row blocks or tiles; products and scales on
  * the 8-bit tensor cores, which add 32 products at a time to an fp32 sum and truncate it, over ranges of K of
  * at most 1024 (fp32 outputs) or 2560 (16-bit ones); the ranges are added in fp32, to nearest. bias (fp32 [N]) may be NULL. activation: enum

@@ -52,6 +52,10 @@ class SfBlocks(_c.Structure):
                 ("tile", _c.c_int32), ("reserved", _c.c_int32)]
 
 
+class SfBlockPlan(_c.Structure):
+    _fields_ = [("tile_rows", _c.c_int32), ("tile_cols", _c.c_int32), ("splits", _c.c_int32), ("range", _c.c_int32)]
+
+
 _BP = _c.POINTER(SfBlocks)
 _MP = _c.POINTER(SfMatrix)
 _VP = _c.POINTER(SfVector)
@@ -89,6 +93,7 @@ SIGNATURES = {
     "sf_blocks_quantize_workspace": (_c.c_int, [_MP, _c.c_int, _SIZE_P]),
     "sf_blocks_quantize": (_c.c_int, [_MP, _BP, _BP, _P, _P, _c.c_size_t, _P]),
     "sf_block_matmul_workspace": (_c.c_int, [_BP, _BP, _MP, _SIZE_P]),
+    "sf_block_matmul_plan": (_c.c_int, [_BP, _BP, _MP, _c.POINTER(SfBlockPlan)]),
     "sf_block_matmul": (_c.c_int, [_BP, _BP, _P, _P, _c.c_int, _MP, _P, _c.c_size_t, _P]),
     "sf_linear8_bytes": (_c.c_int, [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _SIZE_P, _SIZE_P,
                                     _SIZE_P]),

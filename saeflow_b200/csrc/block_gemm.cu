@@ -996,6 +996,20 @@ int sf_block_matmul_workspace(const sf_blocks *a, const sf_blocks *b, const sf_m
     return SF_OK;
 }
 
+int sf_block_matmul_plan(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out, sf_block_plan *plan) {
+    const int st = check_product(a, b, out);
+    if (st) return st;
+    if (!plan) return set_error(SF_ERR_INVALID, "plan is NULL");
+    *plan = sf_block_plan{};
+    if (out->rows == 0 || out->cols == 0) return SF_OK;
+    const Plan pl = make_plan(a->rows, b->rows, a->cols, out->dtype);
+    plan->tile_rows = pl.pair ? 256 : pl.cols;
+    plan->tile_cols = pl.pair ? kPairCols : kRowTile;
+    plan->splits = pl.splits;
+    plan->range = (int)std::min<int64_t>(a->cols, (int64_t)pl.range_groups * 4 * kKBytes);
+    return SF_OK;
+}
+
 int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, const float *threshold, int activation,
                     const sf_matrix *out, void *workspace, size_t workspace_bytes, sf_stream stream) {
     size_t need = 0;

@@ -221,6 +221,15 @@ def block_matmul(a, b, bias=None, activation=None, threshold=None, *, out_dtype=
     return out
 
 
+def product_plan(a, b, out_dtype=torch.bfloat16):
+    """How block_matmul computes a @ b.T: (rows, columns of a tile, splits of K, K of a sum in the tensor cores)."""
+    plan = _abi.SfBlockPlan()
+    out = _abi.SfMatrix(a._c.data, _abi.dtype_code(out_dtype, "out_dtype"), 0, a.shape[0], b.shape[0], b.shape[0], 1)
+    with torch.cuda.device(a.device):
+        _abi.check(_abi.load().sf_block_matmul_plan(a._ref, b._ref, ctypes.byref(out), ctypes.byref(plan)))
+    return plan.tile_rows, plan.tile_cols, plan.splits, plan.range
+
+
 def _vector(v, name, n, dev):
     """A [n] vector in contiguous fp32, or None."""
     if v is None:
