@@ -38,7 +38,13 @@ class BlockScaled:
       2^(s - 127).
     """
 
-    __slots__ = ("data", "scales", "tile", "shape", "device", "_ref", "_c")
+    __slots__ = ("_data", "_scales", "_tile", "_shape", "_device", "_ref", "_c")
+    # What the library reads is in _c, with the tensors' addresses: a matrix is made anew, not changed.
+    data = property(lambda self: self._data)
+    scales = property(lambda self: self._scales)
+    tile = property(lambda self: self._tile)
+    shape = property(lambda self: self._shape)
+    device = property(lambda self: self._device)
 
     def __init__(self, data, scales, tile=False):
         if data.dim() != 2 or scales.dim() != 2:
@@ -47,7 +53,7 @@ class BlockScaled:
             raise ValueError(f"data has dtype {data.dtype}; expected float8_e4m3fn")
         if scales.dtype != torch.uint8:
             raise ValueError(f"scales has dtype {scales.dtype}; expected uint8")
-        self.device = _abi.require_cuda(("data", data), ("scales", scales))
+        self._device = _abi.require_cuda(("data", data), ("scales", scales))
         R, K = data.shape
         want = (_cdiv(R, BLOCK) if tile else R, _cdiv(K, BLOCK))
         if tuple(scales.shape) != want:
@@ -58,11 +64,11 @@ class BlockScaled:
                               or t.shape[0] > 1 and t.stride(0) < t.shape[1] or t.data_ptr() % align):
                 raise ValueError(f"{name} needs a unit column stride and {align}-byte aligned rows, got strides "
                                  f"{t.stride()}")
-        self.data, self.scales, self.tile, self.shape = data, scales, bool(tile), (R, K)
+        self._data, self._scales, self._tile, self._shape = data, scales, bool(tile), (R, K)
         # a single row's stride is never used; any covering multiple passes the library's checks
         dp = data.stride(0) if R > 1 else _cdiv(K, 16) * 16
         sp = scales.stride(0) if scales.shape[0] > 1 else _cdiv(want[1], 4) * 4
-        self._c = _abi.SfBlocks(data.data_ptr(), scales.data_ptr(), R, K, dp, sp, int(self.tile), 0)
+        self._c = _abi.SfBlocks(data.data_ptr(), scales.data_ptr(), R, K, dp, sp, int(self._tile), 0)
         self._ref = ctypes.byref(self._c)
 
     @classmethod
@@ -77,8 +83,8 @@ class BlockScaled:
         # a product reads scale bytes four at a time, so the padding is there; its values are never used
         scales = torch.empty(scale_rows, sp, dtype=torch.uint8, device=dev)
         self = cls.__new__(cls)
-        self.data, self.scales = data, scales if sp == nb else scales[:, :nb]
-        self.tile, self.shape, self.device = bool(tile), (rows, cols), data.device
+        self._data, self._scales = data, scales if sp == nb else scales[:, :nb]
+        self._tile, self._shape, self._device = bool(tile), (rows, cols), data.device
         self._c = _abi.SfBlocks(data.data_ptr(), scales.data_ptr(), rows, cols, dp, sp, int(tile), 0)
         self._ref = ctypes.byref(self._c)
         return self
