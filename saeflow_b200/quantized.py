@@ -4,6 +4,10 @@
 
 x stays as the store holds it, so the b_dec shift moves into the bias, taken with the quantised
 weights W8 (tiles of 128 x 128) that the product uses. Decoding is the 16 / 32-bit path unchanged.
+
+A NaN pre-activation (a row that was stored with an infinity or NaN) is an inactive feature, as in SAE.encode and
+encode_sparse: `pre > 0` is false. block_matmul's own "relu" keeps the NaN, so ReLU is its "jumprelu" with
+thresholds of 0 here (4096 x 768 x 16384: bf16 68.7 against 69.7 us, fp32 81 against 89).
 """
 
 from __future__ import annotations
@@ -29,14 +33,15 @@ class QuantizedSAE:
         self.w8 = quantize(sae.W_enc.detach(), tile=True, transpose=True)  # [d_sae, d_in]
         shift = matvec(self.w8.dequantize(torch.float32), sae.b_dec.detach().float())
         self.bias = sae.b_enc.detach().float() - shift
-        self.threshold = sae.threshold.detach().float() if sae.activation == "jumprelu" else None
+        self.threshold = (sae.threshold.detach().float() if sae.activation == "jumprelu"
+                          else torch.zeros_like(self.bias))
         self.W_dec, self.b_dec = sae.W_dec.detach(), sae.b_dec.detach()
 
     def encode(self, x8, dtype=None):
         """Dense features [M, d_sae] of x8 (BlockScaled [M, d_in], row blocks), in `dtype` (default W_dec's)."""
         if not isinstance(x8, BlockScaled):
             raise ValueError("QuantizedSAE encodes BlockScaled activations (store.take, store.view, quantize)")
-        return block_matmul(x8, self.w8, self.bias, self.activation, self.threshold,
+        return block_matmul(x8, self.w8, self.bias, "jumprelu", self.threshold,
                             out_dtype=dtype or self.W_dec.dtype)
 
     def encode_sparse(self, x8, dtype=None):

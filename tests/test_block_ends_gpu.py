@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import saeflow_b200
 from saeflow_b200.kernels import device_error, quantize
 from saeflow_b200.store import ActivationStore
 
@@ -25,3 +26,25 @@ def test_a_matrix_keeps_the_tensors_it_was_made_of():
             with pytest.raises(AttributeError):
                 setattr(blocks, name, getattr(other, name))
         assert blocks._c.data == blocks.data.data_ptr() and blocks._c.scales == blocks.scales.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("activation", ["relu", "jumprelu"])
+@pytest.mark.parametrize("rows", [7, 1000])
+def test_rows_that_are_not_finite_have_no_features(rows, activation, dtype):
+    """As in the 16 and 32-bit encoders: a NaN pre-activation is no feature, whatever the activation."""
+    sae = saeflow_b200.SAE(200, 3000, activation, device="cuda", dtype=dtype)
+    if activation == "jumprelu":
+        sae.threshold.uniform_(0.1, 0.2)
+    x = torch.randn(rows, 200, device="cuda", dtype=dtype)
+    x[3, 17] = float("nan")
+    x[5, 100] = float("inf")
+    x8 = quantize(x)
+    q = saeflow_b200.QuantizedSAE(sae)
+    plain = x.clone()
+    plain[5] = float("nan")  # as the row is held: at least one NaN
+    assert (saeflow_b200.encode(sae, plain)[[3, 5]] == 0).all()  # the framework's rule
+    f = q.encode(x8)
+    assert (f[[3, 5]] == 0).all() and torch.isfinite(f).all() and (f != 0).any(1).sum() == rows - 2
+    indptr, _, values = q.encode_sparse(x8)
+    assert indptr[4] == indptr[3] and indptr[6] == indptr[5] and torch.isfinite(values).all()
