@@ -405,7 +405,7 @@ SF_API int sf_linear8_forward(const sf_matrix *x, const sf_matrix *W, const floa
                               void *keep, void *temp, size_t temp_bytes, sf_stream stream);
 
 /*
- * From dy [M, N] (M > 0): dx [M, K] = Q(dy) @ Q(W)^T, dW [K, N] = Q(x^T) @ Q(dy^T)^T and db fp32 [N], the
+ * From dy [M, N] (M > 0; with N = 0 dx is zeros): dx [M, K] = Q(dy) @ Q(W)^T, dW [K, N] = Q(x^T) @ Q(dy^T)^T and db fp32 [N], the
  * sums of dy over its rows; NULL where not wanted (`needs` is the forward's, which laid out `keep`).
  */
 SF_API int sf_linear8_backward(const sf_matrix *dy, const void *keep, int64_t K, int needs, const sf_matrix *dx,

@@ -83,7 +83,7 @@ int sf_linear8_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int W_dtype, 
     if ((st = product_bytes(xq, wt, like(M, N, x_dtype), &ws))) return st;
     *forward_temp = fc.used + up256(ws);
     *backward_temp = 0;
-    if (M == 0) return SF_OK;
+    if (M == 0 || N == 0) return SF_OK;
     size_t wx = 0, ww = 0;
     const sf_blocks dyq = bc.blocks(M, N, false);
     if ((needs & kNeedX) && (st = product_bytes(dyq, k.wq, like(M, K, x_dtype), &wx))) return st;
@@ -123,6 +123,16 @@ int sf_linear8_backward(const sf_matrix *dy, const void *keep, int64_t K, int ne
     if (M == 0) return set_error(SF_ERR_INVALID, "dy has no rows");
     if ((dx && !(needs & kNeedX)) || (dW && !(needs & kNeedW)))
         return set_error(SF_ERR_INVALID, "a gradient that the forward kept nothing for");
+    if (N == 0) {  // no features: dx is zeros, dW and db are empty
+        if (!dx) return SF_OK;
+        if (dx->rows != M || dx->cols != K || !dx->data || !sf::valid_dtype(dx->dtype))
+            return set_error(SF_ERR_INVALID, "dx must be [M, K]");
+        if (dx->stride_col != 1 || dx->stride_row < K) return set_error(SF_ERR_UNSUPPORTED, "dx needs a unit column stride");
+        const size_t es = sf::dtype_size(dx->dtype);
+        return sf::check_cuda(cudaMemset2DAsync(const_cast<void *>(dx->data), (size_t)dx->stride_row * es, 0, (size_t)K * es,
+                                                (size_t)M, reinterpret_cast<cudaStream_t>(stream)),
+                              "dx of no features");
+    }
     Carver kc{static_cast<char *>(const_cast<void *>(keep))}, tc{static_cast<char *>(temp)};
     const Kept k = lay_out_keep(kc, M, K, N, needs);
     if (kc.used && !keep) return set_error(SF_ERR_INVALID, "keep is NULL");

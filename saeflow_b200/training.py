@@ -136,7 +136,8 @@ def linear8(x, W, b=None):
     computes (y and dx: x's, dW: W's):
         y  = Q(x) @ Q(W) + b        dx = Q(dy) @ Q(W)^T
         dW = Q(x^T) @ Q(dy^T)^T     db = sum_rows dy   (dy as it is, fp32, in a fixed order)
-    The quantisation itself is taken as the identity (straight through); once differentiable."""
+    The quantisation itself is taken as the identity (straight through); once differentiable. M and N may be 0,
+    K may not."""
     if x.dim() != 2 or W.dim() != 2 or x.shape[1] != W.shape[0]:
         raise ValueError(f"linear8 takes x [M, K] and W [K, N], got {tuple(x.shape)} and {tuple(W.shape)}")
     if b is not None and tuple(b.shape) != (W.shape[1],):

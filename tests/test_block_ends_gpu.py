@@ -6,6 +6,7 @@ import torch
 import saeflow_b200
 from saeflow_b200.kernels import device_error, quantize
 from saeflow_b200.store import ActivationStore
+from saeflow_b200.training import linear8
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +49,22 @@ def test_rows_that_are_not_finite_have_no_features(rows, activation, dtype):
     assert (f[[3, 5]] == 0).all() and torch.isfinite(f).all() and (f != 0).any(1).sum() == rows - 2
     indptr, _, values = q.encode_sparse(x8)
     assert indptr[4] == indptr[3] and indptr[6] == indptr[5] and torch.isfinite(values).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [1, 300])
+def test_linear8_without_features(M, dtype):
+    """N = 0: an empty output, a gradient of zeros for x, empty ones for W and b; for every set of wanted gradients."""
+    for wanted in range(8):
+        x, W, b = (torch.randn(*s, device="cuda", dtype=t).requires_grad_(bool(wanted >> i & 1))
+                   for i, (s, t) in enumerate((((M, 100), dtype), ((100, 0), dtype), ((0,), torch.float32))))
+        with torch.no_grad():
+            assert linear8(x, W, b).shape == (M, 0)
+        y = linear8(x, W, b)
+        assert y.shape == (M, 0) and y.dtype == dtype and y.requires_grad == bool(wanted)
+        if wanted:
+            torch.full((1 << 20,), float("nan"), device="cuda")  # what freed memory may hold
+            y.sum().backward()
+        for i, (t, shape) in enumerate(((x, (M, 100)), (W, (100, 0)), (b, (0,)))):
+            if wanted >> i & 1:
+                assert t.grad.shape == shape and t.grad.dtype == t.dtype and (t.grad == 0).all()
