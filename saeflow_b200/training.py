@@ -27,6 +27,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .kernels import sparse_decode
 from .kernels.backward import csc_gather, csr_sddmm, csr_transpose, matvec, transpose
@@ -143,5 +144,7 @@ def linear8(x, W, b=None):
     if b is not None and tuple(b.shape) != (W.shape[1],):
         raise ValueError(f"b must be [{W.shape[1]}], got {tuple(b.shape)}")
     if not torch.is_grad_enabled():  # only the product: nothing is laid out for a backward
+        if any(t is not None and unpack_dual(t).tangent is not None for t in (x, W, b)):  # they stay on under no_grad
+            raise NotImplementedError("linear8 has no forward-mode derivative")
         return linear8_forward(x, W, b, 0)[0]
     return _Linear8.apply(x, W, b)

@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import saeflow_b200
 from saeflow_b200.kernels import device_error, quantize
@@ -68,3 +69,18 @@ def test_linear8_without_features(M, dtype):
         for i, (t, shape) in enumerate(((x, (M, 100)), (W, (100, 0)), (b, (0,)))):
             if wanted >> i & 1:
                 assert t.grad.shape == shape and t.grad.dtype == t.dtype and (t.grad == 0).all()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_linear8_refuses_forward_mode(which, grad):
+    """Tangents stay on under no_grad: they are refused in both modes, not dropped."""
+    args = [torch.randn(*s, device="cuda") for s in ((5, 64), (64, 32), (32,))]
+    want = linear8(*args)
+    with forward_ad.dual_level():
+        dual = list(args)
+        dual[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with torch.set_grad_enabled(grad):
+            assert torch.equal(linear8(*args), want)
+            with pytest.raises(NotImplementedError, match="forward.mode"):
+                linear8(*dual)
