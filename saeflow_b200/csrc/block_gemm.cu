@@ -905,7 +905,8 @@ struct Plan {
     int range_groups;  // groups of 512 of K to a sum in TMEM
 };
 
-int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int cdiv(int64_t a, int64_t b) { return (int)cdiv64(a, b); }
 
 Plan make_plan(int64_t M, int64_t N, int64_t K, int out_dtype) {
     Plan pl{};
@@ -916,9 +917,9 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int out_dtype) {
     // single): 256 x 768 x 16384 11.8 / 16.8, 512 x 512 x 5000 8.7 / 13.7, 2048 x 1024 x 2048 11.3 / 16.0, and
     // about even where both fit one wave (200 x 768 x 5000: 9.6 / 9.7).
     const int cols = M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t one_tiles = (int64_t)cdiv(N, 128) * cdiv(M, cols);
-    const int64_t pair_tiles = (int64_t)cdiv(N, 256) * cdiv(M, 256);
-    const int64_t one_cost = cdiv(one_tiles, sms) * (int64_t)(128 + cols), pair_cost = cdiv(pair_tiles, sms / 2) * 256;
+    const int64_t one_tiles = cdiv64(N, 128) * cdiv64(M, cols);
+    const int64_t pair_tiles = cdiv64(N, 256) * cdiv64(M, 256);
+    const int64_t one_cost = cdiv64(one_tiles, sms) * (128 + cols), pair_cost = cdiv64(pair_tiles, sms / 2) * 256;
     pl.pair = M > 128 && pair_cost < one_cost;
     pl.cols = pl.pair ? kPairCols : cols;
     const int64_t tiles = pl.pair ? pair_tiles : one_tiles;
@@ -953,8 +954,16 @@ int check_product(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out) 
     // int coordinates, up to a tile past the end
     constexpr int64_t most = INT32_MAX - 4096;
     if (a->rows > most || b->rows > most || a->cols > most) return set_error(SF_ERR_UNSUPPORTED, "extent too large");
-    if ((int64_t)cdiv(a->rows, 32) * cdiv(b->rows, 128) > INT32_MAX / 512)
-        return set_error(SF_ERR_UNSUPPORTED, "too many output tiles");
+    return SF_OK;
+}
+
+// Checks a product of which something is asked for and plans it. Its tiles, over all splits, are numbered in 32
+// bits, and a step of the grid past the last.
+int plan_product(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out, Plan *pl) {
+    *pl = make_plan(a->rows, b->rows, a->cols, out->dtype);
+    const int64_t tiles = pl->pair ? cdiv64(b->rows, kPairCols) * cdiv64(a->rows, 256)
+                                   : cdiv64(b->rows, kRowTile) * cdiv64(a->rows, pl->cols);
+    if (tiles * pl->splits > INT32_MAX - 65536) return set_error(SF_ERR_UNSUPPORTED, "too many output tiles");
     return SF_OK;
 }
 
@@ -986,23 +995,25 @@ using namespace sf;
 extern "C" {
 
 int sf_block_matmul_workspace(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out, size_t *bytes) {
-    const int st = check_product(a, b, out);
+    int st = check_product(a, b, out);
     if (st) return st;
     if (!bytes) return set_error(SF_ERR_INVALID, "bytes is NULL");
     *bytes = 0;
     if (out->rows == 0 || out->cols == 0) return SF_OK;
-    const Plan pl = make_plan(a->rows, b->rows, a->cols, out->dtype);
+    Plan pl;
+    if ((st = plan_product(a, b, out, &pl))) return st;
     if (pl.splits > 1) *bytes = (size_t)pl.splits * out->rows * partial_pitch(out->cols) * sizeof(float);
     return SF_OK;
 }
 
 int sf_block_matmul_plan(const sf_blocks *a, const sf_blocks *b, const sf_matrix *out, sf_block_plan *plan) {
-    const int st = check_product(a, b, out);
+    int st = check_product(a, b, out);
     if (st) return st;
     if (!plan) return set_error(SF_ERR_INVALID, "plan is NULL");
     *plan = sf_block_plan{};
     if (out->rows == 0 || out->cols == 0) return SF_OK;
-    const Plan pl = make_plan(a->rows, b->rows, a->cols, out->dtype);
+    Plan pl;
+    if ((st = plan_product(a, b, out, &pl))) return st;
     plan->tile_rows = pl.pair ? 256 : pl.cols;
     plan->tile_cols = pl.pair ? kPairCols : kRowTile;
     plan->splits = pl.splits;
@@ -1022,9 +1033,8 @@ int sf_block_matmul(const sf_blocks *a, const sf_blocks *b, const float *bias, c
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
         return set_error(SF_ERR_WORKSPACE, "16-byte aligned workspace of %zu bytes needed", need);
     const int M = (int)a->rows, N = (int)b->rows;
-    const Plan pl = make_plan(M, N, a->cols, out->dtype);
-    if ((int64_t)cdiv(M, 32) * cdiv(N, 128) * pl.splits > INT32_MAX / 2)
-        return set_error(SF_ERR_UNSUPPORTED, "too many output tiles and ranges of K");
+    Plan pl;
+    if ((st = plan_product(a, b, out, &pl))) return st;
     // Partial sums go to the workspace in fp32, without bias or activation, and are joined after.
     const bool partial = pl.splits > 1;
     sf_matrix dst = *out;

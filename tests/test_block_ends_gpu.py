@@ -5,7 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 import saeflow_b200
-from saeflow_b200.kernels import device_error, quantize
+from saeflow_b200.kernels import block_matmul, device_error, quantize
 from saeflow_b200.store import ActivationStore
 from saeflow_b200.training import linear8
 
@@ -84,3 +84,13 @@ def test_linear8_refuses_forward_mode(which, grad):
             assert torch.equal(linear8(*args), want)
             with pytest.raises(NotImplementedError, match="forward.mode"):
                 linear8(*dual)
+
+
+def test_a_product_of_very_many_rows():
+    """More than 2^22 tiles of rows, offsets past 32 bits in the operand and the output; small integers, exact."""
+    M = 134217800
+    a = torch.randint(-3, 4, (M, 4), device="cuda", dtype=torch.int8).bfloat16()
+    b = torch.tensor([[1.0, -2.0, 3.0, 1.0]], device="cuda", dtype=torch.bfloat16)
+    got = block_matmul(quantize(a), quantize(b))
+    for i in range(0, M, 1 << 24):
+        assert torch.equal(got[i:i + (1 << 24)], a[i:i + (1 << 24)] @ b.T)

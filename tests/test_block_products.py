@@ -34,3 +34,16 @@ def test_sums_are_never_longer_than_their_type_allows(K):
     for M, N in ((4096, 4096), (1, 64), (640, 640)):
         for dtype, most in ((_abi.SF_F32, 1024), (_abi.SF_BF16, 2560), (_abi.SF_F16, 2560)):
             assert plan(M, N, K, dtype)[3] <= min(most, K)
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(262144, 65536, 2304, _abi.SF_BF16), (1 << 20, 16384, 768, _abi.SF_BF16),
+                                         (65536, 1 << 20, 16384, _abi.SF_F32), (134217800, 1, 16, _abi.SF_BF16)])
+def test_large_outputs_are_planned(M, N, K, dtype):
+    """Tens of GB of output: tiles are counted as they are cut, up to what 32 bits number."""
+    assert plan(M, N, K, dtype)[0] in (128, 256)
+
+
+@pytest.mark.parametrize("M,N", [(1 << 30, 1 << 30), ((1 << 31) - 5000, (1 << 31) - 5000), (1 << 25, 1 << 24)])
+def test_too_many_tiles_are_refused(M, N):
+    with pytest.raises(RuntimeError, match="too many output tiles"):
+        plan(M, N, 128, _abi.SF_BF16)
