@@ -656,7 +656,7 @@ int sf_blocks_read(const sf_blocks *src, const int64_t *rows, const sf_matrix *o
     if (out->cols != src->cols) return set_error(SF_ERR_INVALID, "out and src differ in columns");
     if (!rows && out->rows > src->rows) return set_error(SF_ERR_INVALID, "out has more rows than src");
     if (out->rows == 0 || out->cols == 0) return SF_OK;
-    if (out->stride_col != 1) return set_error(SF_ERR_UNSUPPORTED, "out needs a unit column stride");
+    if (out->cols > 1 && out->stride_col != 1) return set_error(SF_ERR_UNSUPPORTED, "out needs a unit column stride");
     if (out->cols > INT32_MAX - 4096) return set_error(SF_ERR_UNSUPPORTED, "too many columns");
     const bool aligned = vector_rows(*out);
     // a row's pieces of eight, one more where rows start between boundaries

@@ -94,3 +94,14 @@ def test_a_product_of_very_many_rows():
     got = block_matmul(quantize(a), quantize(b))
     for i in range(0, M, 1 << 24):
         assert torch.equal(got[i:i + (1 << 24)], a[i:i + (1 << 24)] @ b.T)
+
+
+def test_read_into_one_column_of_a_row_major_tensor():
+    """A single column's own stride is never used."""
+    store = ActivationStore(50, 1)
+    x = torch.randn(50, 1, device="cuda")
+    store.append(x)
+    wide = torch.full((3, 50), 7.0, device="cuda")
+    store.read(torch.arange(50, device="cuda"), out=wide.T[:, 1:2])
+    assert torch.equal(wide[1:2].T, store.read(torch.arange(50, device="cuda"), torch.float32))
+    assert (wide[[0, 2]] == 7).all()
