@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(256, sizeof(XT) == 4 ? 2 : TILE ? 4 : 3)
     __shared__ uint32_t col_max[8][kBlk / PER];
     __shared__ uint32_t warp_max[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 7;
-    const int64_t rb = blockIdx.y, cb = blockIdx.x;
+    const int64_t rb = blockIdx.y + (int64_t)gridDim.y * blockIdx.z, cb = blockIdx.x;
+    if (rb * kBlk >= R) return;
     const int rl = 16 * warp + 4 * (lane >> 3);
     const int64_t r0 = rb * kBlk + rl, c0 = cb * kBlk + 16 * l;
 
@@ -726,7 +727,9 @@ int sf_blocks_quantize(const sf_matrix *x, const sf_blocks *q, const sf_blocks *
     if (need && (!workspace || workspace_bytes < need))
         return set_error(SF_ERR_WORKSPACE, "workspace of %zu bytes needed", need);
     const int64_t nrb = (x->rows + kBlk - 1) / kBlk, ncb = (x->cols + kBlk - 1) / kBlk;
-    if (nrb > 65535) return set_error(SF_ERR_UNSUPPORTED, "too many rows for one call");
+    // row blocks along y and z, at most 65535 either way; blocks past the last leave at once
+    const int64_t ny = std::min<int64_t>(nrb, 32768), nz = (nrb + ny - 1) / ny;
+    if (nz > 65535 || ncb > INT32_MAX) return set_error(SF_ERR_UNSUPPORTED, "too many rows or columns for one call");
     const bool tile = (q ? q : qt)->tile != 0;
     float *part = col_sums ? static_cast<float *>(workspace) : nullptr;
     const sf_blocks none = {};
@@ -734,7 +737,7 @@ int sf_blocks_quantize(const sf_matrix *x, const sf_blocks *q, const sf_blocks *
     st = with_type(x->dtype, [&](auto tag) {
         using T = decltype(tag);
         auto kern = tile ? quant_tile_kernel<T, true> : quant_tile_kernel<T, false>;
-        kern<<<dim3((unsigned)ncb, (unsigned)nrb), 256, 0, s>>>(
+        kern<<<dim3((unsigned)ncb, (unsigned)ny, (unsigned)nz), 256, 0, s>>>(
             reinterpret_cast<const T *>(x->data), x->rows, x->cols, x->stride_row, x->stride_col, vector_rows(*x),
             static_cast<uint8_t *>(a.data), a.data_pitch, static_cast<uint8_t *>(a.scales), a.scale_pitch,
             static_cast<uint8_t *>(b.data), b.data_pitch, static_cast<uint8_t *>(b.scales), b.scale_pitch, part);

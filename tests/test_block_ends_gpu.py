@@ -5,7 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 import saeflow_b200
-from saeflow_b200.kernels import block_matmul, device_error, quantize
+from saeflow_b200.kernels import block_matmul, device_error, quantize, quantize_both
 from saeflow_b200.store import ActivationStore
 from saeflow_b200.training import linear8
 
@@ -105,3 +105,22 @@ def test_read_into_one_column_of_a_row_major_tensor():
     store.read(torch.arange(50, device="cuda"), out=wide.T[:, 1:2])
     assert torch.equal(wide[1:2].T, store.read(torch.arange(50, device="cuda"), torch.float32))
     assert (wide[[0, 2]] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantising_very_many_rows(dtype):
+    """More row blocks than a grid's second extent (65535 x 128 rows): in tiles, transposed and with column sums."""
+    R, C = 65535 * 128 + 300, 5
+    x = torch.randint(-8, 9, (R, C), device="cuda", dtype=torch.int8).to(dtype)
+    x[-200:] *= 64
+    q, qt, sums = quantize_both(x, col_sums=True)
+    rows = quantize(x)
+    assert torch.equal(q.data.view(torch.uint8), rows.data.view(torch.uint8)) and torch.equal(q.scales, rows.scales)
+    want = quantize(x.T.contiguous())
+    assert torch.equal(qt.data.view(torch.uint8), want.data.view(torch.uint8)) and torch.equal(qt.scales, want.scales)
+    assert torch.equal(sums.double(), x.double().sum(0))  # small integers: exact in any order
+    t = quantize(x, tile=True)
+    first = R // 128 * 128 - 128 * 5
+    last = quantize(x[first:], tile=True)
+    assert torch.equal(t.data[first:].view(torch.uint8), last.data.view(torch.uint8))
+    assert torch.equal(t.scales[first // 128:], last.scales)
