@@ -1396,25 +1396,25 @@ int make_map_out(CUtensorMap *map, const void *base, int dtype, uint64_t cols, u
     return SF_OK;
 }
 
-// Pairs of SMs that can hold one pair-kernel cluster each (cached per kernel).
+// Pairs of SMs of the current device that can hold one pair-kernel cluster each (kept per kernel and device; a query
+// that failed is asked again).
 int pair_slots(const void *kern, const cudaLaunchConfig_t &cfg) {
     static std::mutex mu;
-    static const void *keys[64];
-    static int vals[64];
+    static struct {
+        const void *kern;
+        int device, clusters;
+    } kept[512];
     static int n = 0;
+    int device = 0, clusters = 0;
+    cudaGetDevice(&device);
     std::lock_guard<std::mutex> lk(mu);
     for (int i = 0; i < n; ++i)
-        if (keys[i] == kern) return vals[i];
-    int clusters = 0;
+        if (kept[i].kern == kern && kept[i].device == device) return kept[i].clusters;
     if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess || clusters <= 0) {
         cudaGetLastError();
-        clusters = std::max(1, num_sms() / 2);
+        return std::max(1, num_sms() / 2);
     }
-    if (n < 64) {
-        keys[n] = kern;
-        vals[n] = clusters;
-        ++n;
-    }
+    if (n < 512) kept[n++] = {kern, device, clusters};
     return clusters;
 }
 
