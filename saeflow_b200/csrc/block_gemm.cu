@@ -33,12 +33,14 @@
 // What bounds it. A pair reads 64 KB of operands from L2 per K block; all 148 SMs together get about 6 KB a
 // clock, 700 to 780 clocks a block, where the MMAs take 512 (530 measured with the loads left out): large
 // products are bound by operand delivery, and in a steady loop by the 1000 W power cap (SM clock near
-// 1.4 GHz). Few rows of `a` are bound by the bytes of `b`, K below some 1500 by the epilogue (about 3300
-// clocks a tile). Two accumulators of 256 columns and the scales exceed TMEM, so the accumulators overlap;
+// 1.4 GHz). Few rows of `a` are bound by the bytes of `b`; K below some 1500 by the handoff of tiles: the epilogue
+// takes about 3300 clocks a tile, and at K = 768 waits another 1050 to 1440 for the next one's sums while the MMA
+// warp waits about 3000 for its accumulator. Two accumulators of 256 columns and the scales exceed TMEM, so the accumulators overlap;
 // 224-column tiles, whose accumulators do not, move 7% more bytes and were slower at every K from 128 up.
 // Measured on a B200, bf16 outputs (M x K x N): 16384 x 2304 x 65536 1.95 ms, 2.5 PFLOP/s (in a steady loop 2.3 ms,
-// 2.15 PFLOP/s, 0.92 of the library's 8-bit product with one scale per tensor); 4096 x 768 x 16384 66 us;
-// 1 x 2304 x 65536 30.5 us, 5.0 TB/s of weights.
+// 2.15 PFLOP/s, 0.92 of the library's 8-bit product with one scale per tensor); 4096 x 8192 x 16384 395 us, 2.8
+// PFLOP/s, tensor pipe 77%; 16384 x 768 x 65536 985 us, 1.7 PFLOP/s; 4096 x 768 x 16384 58 to 69 us, box to box;
+// 1 x 2304 x 65536 31 us, 4.9 TB/s of weights.
 #include <algorithm>
 #include <type_traits>
 
@@ -928,7 +930,8 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int out_dtype) {
     // second kernel. Measured (us, split against whole): K = 768 12.7 / 9.5 (512 x 2048), 2304 13.0 / 12.4
     // (256 x 2048), 5000 19.3 / 23.6 (1000 x 768), 8192 16.1 / 24.4 (640 x 640), 13558 23.5 / 35.1 (636 x 1094).
     pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(groups / 4, slots / tiles));
-    // fp32 outputs: splits of at most 8192, whatever the number of tiles.
+    // fp32 outputs: splits of at most 8192, whatever the number of tiles, which is what the workspace query has
+    // always asked for. Their exactness comes from the ranges below.
     if (out_dtype == SF_F32) pl.splits = std::max(pl.splits, cdiv(K, 8192));
     // whole splits: none without a group
     const int split_groups = cdiv(groups, pl.splits);

@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(256, 4) read_rows_kernel(const uint8_t *__rest
     }
 }
 
-// Gather of rows as they are held: one warp per row, bound by HBM (16384 rows of 2304 in 13.7 us, 5.5 TB/s).
+// Gather of rows as they are held: one warp per row, two 4-byte loads to each 8-byte store. 16384 rows of 2304 in
+// 13.7 us, 5.5 TB/s, part of them in L2; 65536 in 67 us, 4.5 TB/s, 0.68 of the copy rate: bound by its loads in flight.
 __global__ void __launch_bounds__(256) take_rows_kernel(const uint8_t *__restrict__ q, int64_t q_pitch,
                                                         const uint8_t *__restrict__ s, int64_t s_pitch,
                                                         int64_t src_rows, int64_t K, unsigned nb,

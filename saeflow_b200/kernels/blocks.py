@@ -203,6 +203,9 @@ def block_matmul(a, b, bias=None, activation=None, threshold=None, *, out_dtype=
     bias: [N] or None. activation: None, "relu" or "jumprelu" (needs `threshold` [N]; 0 unless
       the sum is above it).
     out_dtype: fp32 / bf16 / fp16; out: a tensor to write into, unit column stride.
+
+    ReLU keeps a NaN, JumpReLU makes it 0. The result has no gradient: bias and threshold are taken as they are,
+    without their history (saeflow_b200.training.linear8 is the differentiable product).
     """
     dev = a.device
     if b.device != dev:

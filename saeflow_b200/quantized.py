@@ -21,7 +21,7 @@ from .kernels.blocks import BlockScaled, block_matmul, quantize
 
 class QuantizedSAE:
     """The encode / encode_sparse / decode_sparse / forward of `sae` (ReLU or JumpReLU) on BlockScaled
-    activations. The weights are laid out here, once; build it again after an update of `sae`."""
+    activations, for inference: nothing here has a gradient. The weights are laid out here, once; build it again after an update of `sae`."""
 
     def __init__(self, sae):
         if sae.activation not in ("relu", "jumprelu"):
